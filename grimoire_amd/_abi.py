@@ -115,6 +115,27 @@ class ExpertSwap(C.Structure):
     _fields_ = [("promote_layer", C.c_int32), ("promote_expert", C.c_int32),
                 ("demote_layer", C.c_int32), ("demote_expert", C.c_int32)]
 
+
+class ScoreParams(C.Structure):
+    """grim_score_params"""
+    _fields_ = [("score", C.c_int32), ("n_group", C.c_int32), ("topk_group", C.c_int32),
+                ("group_score", C.c_int32), ("normalize", C.c_int32), ("scaling", C.c_float),
+                ("bias", C.c_void_p)]
+
+
+SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1
+GROUP_MAX, GROUP_TOP2 = 0, 1
+
+
+class BlockNormParams(C.Structure):
+    """grim_block_norm_params"""
+    _fields_ = [("post_weight", C.c_void_p), ("pre_weight", C.c_void_p), ("weight_offset", C.c_float),
+                ("eps", C.c_float), ("residual_scale", C.c_float), ("block_scale", C.c_float),
+                ("gate_kind", C.c_int32), ("gate_sigmoid", C.c_int32)]
+
+
+GATE_NONE, GATE_CHANNEL, GATE_ROW, GATE_FULL = 0, 1, 2, 3
+
 P = C.c_void_p
 I32 = C.c_int
 F32 = C.c_float
@@ -122,6 +143,7 @@ SZ = C.c_size_t
 QWP = C.POINTER(QuantWeight)
 LP = C.POINTER(MoeLayer)
 RPP = C.POINTER(RouteParams)
+I64 = C.c_int64
 
 # name -> (restype, argtypes); must match include/grimoire_moe.h
 SIGNATURES = {
@@ -133,6 +155,7 @@ SIGNATURES = {
     "grimoire_moe_router_topk_bf16_batched": (I32, [P, P, I32, I32, I32, P, P, I32]),
     "grimoire_moe_router_topk_sigmoid": (I32, [P, P, P, I32, I32, I32, P, P, I32, F32]),
     "grimoire_moe_router_topk_group": (I32, [P, P, P, I32, I32, I32, I32, I32, P, P, I32, F32]),
+    "grimoire_moe_router_scores": (I32, [P, C.POINTER(ScoreParams), P, I32, I64, I32, I32, I32, P, P]),
     "grimoire_moe_gate_up": (I32, [P, LP, P, P, P]),
     "grimoire_moe_down": (I32, [P, LP, P, P, P, P]),
     "grimoire_moe_gate_up_shared": (I32, [P, LP, QWP, P, P, P, P, P]),
@@ -155,6 +178,9 @@ SIGNATURES = {
     "grimoire_moe_rmsnorm_residual": (I32, [P, P, P, P, P, P, P, F32, P, P, I32, I32, I32,
                                             F32]),
     "grimoire_rmsnorm_residual": (I32, [P, P, P, P, P, F32, P, P, I32, I32, F32]),
+    "grimoire_block_norm": (I32, [P, C.POINTER(BlockNormParams), P, I32, P, P, I32, I64, P, P, P, I32, I32]),
+    "grimoire_moe_block_norm": (I32, [P, C.POINTER(BlockNormParams), P, I32, P, P, I32, P, P, P, P, P, P, I32,
+                                      I32, I32]),
     "grimoire_moe_ingest_projection": (I32, [P, C.POINTER(ExpertSrc), QWP, I32]),
     "grimoire_moe_ingest_projections": (I32, [P, C.POINTER(ExpertSrc), P, I32, QWP]),
     "grimoire_moe_int4_to_signed": (I32, [P, P, SZ, P, SZ, P, SZ, P, SZ, P]),

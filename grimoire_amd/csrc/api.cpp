@@ -13,6 +13,7 @@
 #include <vector>
 
 #include "../../include/grimoire_moe.h"
+#include "block_norm.hpp"
 #include "common.hpp"
 #include "dispatch.hpp"
 #include "gemm.hpp"
@@ -22,6 +23,7 @@
 #include "ingest.hpp"
 #include "tiered.hpp"
 #include "router.hpp"
+#include "scores.hpp"
 #include "gemv_mx.hpp"
 
 using namespace grim;
@@ -289,6 +291,35 @@ int grimoire_moe_router_topk_group(void* stream, const float* logits, const floa
     return topk_common(stream, a);
 }
 
+int grimoire_moe_router_scores(void* stream, const grim_score_params* p, const void* logits,
+                               int logits_bf16, int64_t row_stride, int tokens, int n_experts,
+                               int top_k, int32_t* out_expert, float* out_weight) {
+    if (tokens <= 0) return GRIM_OK;
+    if (!p || !logits || !out_expert || !out_weight) return fail(GRIM_ERR_ARG, "null pointer");
+    if (p->score != GRIM_SCORE_SOFTMAX && p->score != GRIM_SCORE_SIGMOID)
+        return fail(GRIM_ERR_ARG, "score=%d", p->score);
+    if (n_experts <= 0 || n_experts > kScoresMaxE)
+        return fail(GRIM_ERR_SHAPE, "n_experts=%d (1..%d)", n_experts, kScoresMaxE);
+    if (top_k <= 0 || top_k > kScoresMaxK || top_k > n_experts)
+        return fail(GRIM_ERR_SHAPE, "top_k=%d (1..%d)", top_k, kScoresMaxK);
+    if (row_stride < n_experts) return fail(GRIM_ERR_SHAPE, "row_stride=%lld < n_experts", (long long)row_stride);
+    const int G = p->n_group > 1 ? p->n_group : 1;
+    if (p->n_group < 0 || G > kScoresMaxGroups || n_experts % G)
+        return fail(GRIM_ERR_SHAPE, "n_group=%d must divide n_experts=%d (<= %d groups)", p->n_group,
+                    n_experts, kScoresMaxGroups);
+    if (G > 1) {
+        if (p->topk_group <= 0 || p->topk_group > G) return fail(GRIM_ERR_SHAPE, "topk_group=%d", p->topk_group);
+        if (p->group_score != GRIM_GROUP_MAX && p->group_score != GRIM_GROUP_TOP2)
+            return fail(GRIM_ERR_ARG, "group_score=%d", p->group_score);
+        if (top_k > p->topk_group * (n_experts / G))
+            return fail(GRIM_ERR_SHAPE, "top_k exceeds the experts of the kept groups");
+    }
+    ScoresArgs a{logits, row_stride, logits_bf16 ? 1 : 0, tokens, n_experts, top_k,
+                 p->score == GRIM_SCORE_SIGMOID, p->bias, G, G > 1 ? p->topk_group : 1,
+                 p->group_score == GRIM_GROUP_TOP2, p->normalize, p->scaling, out_expert, out_weight};
+    return status(scores_launch(S(stream), a));
+}
+
 int grimoire_moe_gate_up(void* stream, const grim_moe_layer* L, const int32_t* d_expert,
                          const float* x, float* h) {
     return gemv_common(stream, L, nullptr, nullptr, d_expert, x, h, nullptr, 1);
@@ -439,6 +470,63 @@ int grimoire_rmsnorm_residual(void* stream, float* h, const float* r0, const flo
     NormArgs a{h, nullptr, nullptr, nullptr, r0, r1, weight, weight_offset, out, out_bf,
                tokens, 0, hidden, eps};
     return status(combine_norm_launch(S(stream), a));
+}
+
+static bool aligned(const void* p, uintptr_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+
+// What both forms of the block norm check and share.
+static int block_norm_args(const grim_block_norm_params* p, const void* gate, int gate_bf16, const float* h,
+                           float* h_out, float* out, uint16_t* out_bf, int tokens, int hidden,
+                           BlockNormArgs& a) {
+    if (!p || !h) return fail(GRIM_ERR_ARG, "null pointer");
+    if (hidden <= 0 || hidden % 4 || hidden > kBlockNormMaxHidden)
+        return fail(GRIM_ERR_SHAPE, "hidden=%d (need %% 4, <= %d)", hidden, kBlockNormMaxHidden);
+    if (!h_out && !out && !out_bf) return fail(GRIM_ERR_ARG, "no output");
+    if ((out || out_bf) && !p->pre_weight) return fail(GRIM_ERR_ARG, "out without pre_weight");
+    if (p->gate_kind < GRIM_GATE_NONE || p->gate_kind > GRIM_GATE_FULL)
+        return fail(GRIM_ERR_ARG, "gate_kind=%d", p->gate_kind);
+    if ((p->gate_kind != GRIM_GATE_NONE) != (gate != nullptr))
+        return fail(GRIM_ERR_ARG, "gate_kind=%d and gate do not go together", p->gate_kind);
+    if (!aligned(h, 16) || !aligned(h_out, 16) || !aligned(out, 16) || !aligned(out_bf, 8) ||
+        !aligned(p->post_weight, 8) || !aligned(p->pre_weight, 8) ||
+        !aligned(gate, p->gate_kind == GRIM_GATE_ROW ? (gate_bf16 ? 2 : 4) : (gate_bf16 ? 8 : 16)))
+        return fail(GRIM_ERR_ARG, "fp32 rows 16-byte, bf16 rows 8-byte alignment");
+    a = BlockNormArgs{};
+    a.h = h; a.post_w = p->post_weight; a.pre_w = p->pre_weight;
+    a.offset = p->weight_offset; a.eps = p->eps; a.rs = p->residual_scale; a.bs = p->block_scale;
+    a.gate = gate; a.gate_kind = p->gate_kind; a.gate_bf16 = gate_bf16 ? 1 : 0;
+    a.gate_sigmoid = p->gate_sigmoid ? 1 : 0;
+    a.h_out = h_out; a.out = out; a.out_bf = out_bf; a.T = tokens; a.H = hidden;
+    return GRIM_OK;
+}
+
+int grimoire_block_norm(void* stream, const grim_block_norm_params* p, const void* gate, int gate_bf16,
+                        const float* h, const void* x, int x_bf16, int64_t x_stride, float* h_out,
+                        float* out, uint16_t* out_bf, int tokens, int hidden) {
+    if (tokens <= 0) return GRIM_OK;
+    BlockNormArgs a;
+    if (int r = block_norm_args(p, gate, gate_bf16, h, h_out, out, out_bf, tokens, hidden, a)) return r;
+    if (!x) return fail(GRIM_ERR_ARG, "null x");
+    if (x_stride < hidden || x_stride % 4)
+        return fail(GRIM_ERR_SHAPE, "x_stride=%lld (need >= hidden, %% 4)", (long long)x_stride);
+    if (!aligned(x, x_bf16 ? 8 : 16)) return fail(GRIM_ERR_ARG, "x alignment");
+    a.x = x; a.x_bf16 = x_bf16 ? 1 : 0; a.x_stride = x_stride;
+    return status(block_norm_launch(S(stream), a));
+}
+
+int grimoire_moe_block_norm(void* stream, const grim_block_norm_params* p, const void* gate, int gate_bf16,
+                            const float* h, const uint16_t* routed, int routed_rows,
+                            const int32_t* inverse, const float* route_weight, const float* shared,
+                            float* h_out, float* out, uint16_t* out_bf, int tokens, int top_k, int hidden) {
+    if (tokens <= 0) return GRIM_OK;
+    BlockNormArgs a;
+    if (int r = block_norm_args(p, gate, gate_bf16, h, h_out, out, out_bf, tokens, hidden, a)) return r;
+    if (!routed || !inverse || !route_weight) return fail(GRIM_ERR_ARG, "null routed/inverse/weights");
+    if (top_k <= 0 || top_k > 16) return fail(GRIM_ERR_SHAPE, "top_k=%d (1..16)", top_k);
+    if (routed_rows < 0) return fail(GRIM_ERR_SHAPE, "routed_rows=%d", routed_rows);
+    if (!aligned(routed, 8) || !aligned(shared, 16)) return fail(GRIM_ERR_ARG, "routed/shared alignment");
+    a.routed = routed; a.routed_rows = routed_rows; a.inverse = inverse; a.rw = route_weight; a.shared = shared; a.K = top_k;
+    return status(block_norm_launch(S(stream), a));
 }
 
 static int ingest_common(void* stream, const grim_expert_src* srcs, const int32_t* row0s, int n,

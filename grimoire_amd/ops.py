@@ -296,6 +296,172 @@ def grouped_gemm_i8(w: Weight, N, swiglu, A, a_scale, out, offsets, counts, num_
                                              num_experts), "grouped_gemm_i8")
 
 
+# ------------------------------------------------- router scores, block norms
+
+def _rows(t: torch.Tensor, what: str, width: int, rows: int):
+    """(pointer, is bf16, row stride) of a [rows][width] tensor whose rows may
+    lie apart; bf16 also as int16 bits, as elsewhere in this module."""
+    if t.dim() != 2 or t.shape[0] != rows or t.shape[1] != width:
+        raise _abi.GrimoireError(f"{what}: shape {tuple(t.shape)}, expected ({rows}, {width})")
+    st = t.stride()
+    if st[1] != 1 and width > 1:
+        raise _abi.GrimoireError(f"{what}: elements of a row must be adjacent")
+    return t.data_ptr(), _bf16(t, what), (st[0] if rows > 1 else max(st[0], width))
+
+
+def _bf16(t: torch.Tensor, what: str) -> int:
+    if t.dtype is torch.float32:
+        return 0
+    if t.dtype is torch.bfloat16 or t.dtype is torch.int16:
+        return 1
+    raise _abi.GrimoireError(f"{what}: {t.dtype}, expected float32 or bfloat16")
+
+
+def _flat(t: Optional[torch.Tensor], what: str, shape, dtypes, dev: int):
+    """Pointer of a contiguous tensor of `shape` on device `dev`, or None."""
+    if t is None:
+        return None
+    if t.dtype not in dtypes or t.shape != shape or not t.is_contiguous():
+        raise _abi.GrimoireError(f"{what}: {t.dtype} {tuple(t.shape)}, expected contiguous {tuple(shape)}")
+    if t.get_device() != dev:
+        raise _abi.GrimoireError(f"{what}: on another device than the other tensors")
+    return t.data_ptr()
+
+
+_F32, _I32 = (torch.float32,), (torch.int32,)
+_B16 = (torch.bfloat16, torch.int16)
+_FB16 = _F32 + _B16
+
+
+class _On:
+    """Device `dev` as the current one for a launch on a stream of it."""
+    __slots__ = ("dev", "was")
+
+    def __init__(self, dev: int):
+        self.dev = dev
+
+    def __enter__(self):
+        self.was = torch.cuda.current_device()
+        if self.was != self.dev:
+            torch.cuda.set_device(self.dev)
+
+    def __exit__(self, *a):
+        if self.was != self.dev:
+            torch.cuda.set_device(self.was)
+
+
+def _launch(t: torch.Tensor, stream, fn, what: str, *args):
+    """Call entry point fn(stream, *args) on t's device and check its status."""
+    dev = t.get_device()
+    s = (stream if stream is not None else torch.cuda.current_stream(dev)).cuda_stream
+    if torch.cuda.current_device() == dev:
+        check(fn(s, *args), what)
+    else:
+        with _On(dev):
+            check(fn(s, *args), what)
+
+
+class RouteScores:
+    """grimoire_moe_router_scores: how a layer turns router logits into routes.
+
+    score "softmax" (over all experts) or "sigmoid"; bias fp32 [E] counts for
+    the choice only; n_group > 1 keeps the topk_group groups with the best
+    "max" or "top2" score; the picks' weights are divided by their sum when
+    `normalize`, then multiplied by `scaling`."""
+
+    SCORES = {"softmax": _abi.SCORE_SOFTMAX, "sigmoid": _abi.SCORE_SIGMOID}
+    GROUPS = {"max": _abi.GROUP_MAX, "top2": _abi.GROUP_TOP2}
+
+    def __init__(self, score="softmax", bias: Optional[torch.Tensor] = None, n_group=1, topk_group=1,
+                 group_score="max", normalize=True, scaling=1.0):
+        if score not in self.SCORES or group_score not in self.GROUPS:
+            raise _abi.GrimoireError(f"score {score!r}, group_score {group_score!r}")
+        if bias is not None:
+            _dev(bias)
+            _flat(bias, "bias", (bias.numel(),), _F32, bias.get_device())
+        self.bias = bias
+        self.struct = _abi.ScoreParams(self.SCORES[score], n_group, topk_group, self.GROUPS[group_score],
+                                       int(normalize), float(scaling), _p(bias))
+
+    def __call__(self, logits, out_expert, out_weight, stream=None):
+        """Routes of logits [T][E] (fp32 or bf16, rows may lie apart) into
+        out_expert int32 / out_weight fp32 [T][K]."""
+        _dev(logits)
+        dev = logits.get_device()
+        if out_expert.dim() != 2 or logits.dim() != 2:
+            raise _abi.GrimoireError("logits [T][E], out_expert [T][K]")
+        T, K = out_expert.shape
+        E = logits.shape[1]
+        lp, b16, stride = _rows(logits, "logits", E, T)
+        if self.bias is not None and (self.bias.numel() != E or self.bias.get_device() != dev):
+            raise _abi.GrimoireError("bias: one value an expert, on the logits' device")
+        _launch(logits, stream, lib().grimoire_moe_router_scores, "router_scores", self.struct, lp, b16, stride, T, E,
+                K, _flat(out_expert, "out_expert", (T, K), _I32, dev),
+                _flat(out_weight, "out_weight", (T, K), _F32, dev))
+
+
+class BlockNorm:
+    """The norms around one block (grimoire_block_norm): pre_weight of the
+    norm before the next block, post_weight of the norm of this block's
+    output (None: not normed), both bf16 [H]; gate "none", "channel" [H],
+    "row" [T] or "full" [T][H], through a sigmoid with gate_sigmoid."""
+
+    GATES = {"none": _abi.GATE_NONE, "channel": _abi.GATE_CHANNEL, "row": _abi.GATE_ROW, "full": _abi.GATE_FULL}
+
+    def __init__(self, pre_weight: Optional[torch.Tensor], post_weight: Optional[torch.Tensor] = None, eps=1e-6,
+                 weight_offset=1.0, residual_scale=1.0, block_scale=1.0, gate="none", gate_sigmoid=False):
+        if gate not in self.GATES:
+            raise _abi.GrimoireError(f"gate {gate!r}")
+        for w in (pre_weight, post_weight):
+            if w is not None:
+                _dev(w)
+                _flat(w, "norm weight", (w.numel(),), _B16, w.get_device())
+        self.pre_weight, self.post_weight, self.gate = pre_weight, post_weight, gate
+        self.struct = _abi.BlockNormParams(_p(post_weight), _p(pre_weight), float(weight_offset), float(eps),
+                                           float(residual_scale), float(block_scale), self.GATES[gate],
+                                           int(gate_sigmoid))
+
+    def _args(self, h, h_out, out, out_bf, gate):
+        _dev(h)
+        dev = h.get_device()
+        T, H = h.shape
+        for w in (self.pre_weight, self.post_weight):
+            if w is not None and (w.numel() != H or w.get_device() != dev):
+                raise _abi.GrimoireError("norm weights: one value a column, on h's device")
+        kind = self.gate
+        if (gate is not None) != (kind != "none"):
+            raise _abi.GrimoireError(f"gate {kind!r} and the gate tensor do not go together")
+        gp, g16 = None, 0
+        if gate is not None:
+            gp = _flat(gate, "gate", (H,) if kind == "channel" else (T,) if kind == "row" else (T, H), _FB16, dev)
+            g16 = int(gate.dtype is not torch.float32)
+        shape = (T, H)
+        return (T, H, dev, gp, g16, _flat(h, "h", shape, _F32, dev), _flat(h_out, "h_out", shape, _F32, dev),
+                _flat(out, "out", shape, _F32, dev), _flat(out_bf, "out_bf", shape, _B16, dev))
+
+    def __call__(self, h, x, h_out, out=None, out_bf=None, gate=None, stream=None):
+        """Behind a dense block: x [T][H] fp32 or bf16, rows may lie apart."""
+        T, H, dev, gp, g16, hp, hop, op, obp = self._args(h, h_out, out, out_bf, gate)
+        xp, x16, stride = _rows(x, "x", H, T)
+        if x.get_device() != dev:
+            raise _abi.GrimoireError("x: on another device than h")
+        _launch(h, stream, lib().grimoire_block_norm, "block_norm", self.struct, gp, g16, hp, xp, x16, stride, hop, op,
+                obp, T, H)
+
+    def moe(self, h, routed, inverse, route_weight, shared, h_out, out=None, out_bf=None, gate=None, stream=None):
+        """Behind routed experts (grimoire_moe_block_norm): routed bf16
+        [R][H] in dispatch order, inverse [T*K], route_weight [T][K]."""
+        T, H, dev, gp, g16, hp, hop, op, obp = self._args(h, h_out, out, out_bf, gate)
+        if route_weight.dim() != 2:
+            raise _abi.GrimoireError("route_weight: [T][K]")
+        K = route_weight.shape[1]
+        _launch(h, stream, lib().grimoire_moe_block_norm, "moe_block_norm", self.struct, gp, g16, hp,
+                _flat(routed, "routed", (routed.shape[0], H), _B16, dev), routed.shape[0],
+                _flat(inverse.view(-1), "inverse", (T * K,), _I32, dev),
+                _flat(route_weight, "route_weight", (T, K), _F32, dev), _flat(shared, "shared", (T, H), _F32, dev), hop,
+                op, obp, T, K, H)
+
+
 # ------------------------------------------------------------------- layer
 
 class MoeForward:

@@ -164,6 +164,46 @@ int grimoire_moe_router_topk_group(void* stream, const float* logits, const floa
                                    int topk_group, int32_t* out_expert, float* out_weight,
                                    int normalize, float scaling);
 
+/* Router scores in their general form: probabilities over all experts or
+ * sigmoids, a bias that counts for the choice only, groups.  No counterpart
+ * in the reference, whose softmax router weighs the picks alone
+ * (src/ops.cpp:1205).
+ *   s = softmax over the E logits, or sigmoid(l); s' = s + bias (fp32 [E],
+ *   may be NULL).  With n_group > 1 the experts form n_group equal
+ *   contiguous groups (<= 64); a group's score is its largest s', or the sum
+ *   of its two largest (GRIM_GROUP_TOP2; the one there is when only one is
+ *   left), and only the topk_group best groups stay.  The picks are the
+ *   top_k largest s', in descending order; equal values go to the lower
+ *   group / expert index.  weight = s of the pick, divided by the picks' sum
+ *   when `normalize` (0 when that sum is 0), times `scaling`.
+ * An expert is out when its logit is NaN or -inf or its s' is NaN or -inf;
+ * +inf counts as the largest finite logit.  Slots no expert is left for get
+ * expert -1, weight 0 (the products skip such routes).  Scores, sums and the
+ * choice are fp64, so the routing does not depend on fp32 rounding.
+ * logits: fp32 or (logits_bf16) bf16 rows, row_stride elements apart
+ * (>= n_experts).  n_experts <= 512, top_k <= min(16, n_experts), and with
+ * groups <= topk_group * (n_experts / n_group). */
+enum grim_score {
+    GRIM_SCORE_SOFTMAX = 0,
+    GRIM_SCORE_SIGMOID = 1
+};
+enum grim_group_score {
+    GRIM_GROUP_MAX = 0,
+    GRIM_GROUP_TOP2 = 1
+};
+typedef struct grim_score_params {
+    int32_t score;             /* enum grim_score                          */
+    int32_t n_group;           /* 1 (or 0): no group limit                 */
+    int32_t topk_group;        /* groups kept; read when n_group > 1       */
+    int32_t group_score;       /* enum grim_group_score                    */
+    int32_t normalize;
+    float scaling;
+    const float* bias;         /* fp32 [E] or NULL                         */
+} grim_score_params;
+int grimoire_moe_router_scores(void* stream, const grim_score_params* p, const void* logits,
+                               int logits_bf16, int64_t row_stride, int tokens, int n_experts,
+                               int top_k, int32_t* out_expert, float* out_weight);
+
 /* ------------------------------------------------------------------------
  * Decode / batched-decode expert products (slot form).  h holds
  * [M][KS][I] fp32, KS = top_k (+1 with the shared expert, whose
@@ -313,6 +353,53 @@ int grimoire_moe_rmsnorm_residual(void* stream, float* h, const uint16_t* routed
 int grimoire_rmsnorm_residual(void* stream, float* h, const float* r0, const float* r1,
                               const uint16_t* weight, float weight_offset, float* out,
                               uint16_t* out_bf, int tokens, int hidden, float eps);
+
+/* The norms on both sides of a block, its gate and its residual scale in one
+ * pass.  No counterpart in the reference, whose blocks add their output to
+ * the residual stream as it is (src/prefill.cpp:627-700).  Per row t, f the
+ * block's output:
+ *   p  = f * rsqrt(sum(f^2)/hidden + eps) * (weight_offset + post_weight)
+ *        (post_weight NULL: p = f)
+ *   h' = residual_scale * h + block_scale * g * p
+ *   o  = h' * rsqrt(sum(h'^2)/hidden + eps) * (weight_offset + pre_weight)
+ * g = gate, or sigmoid(gate) with gate_sigmoid, fp32 or (gate_bf16) bf16:
+ * one value a channel [hidden], one a row [tokens] or one an element
+ * [tokens][hidden] by gate_kind (GRIM_GATE_NONE: 1, gate is not read).
+ * h_out = h' (may be NULL, may be h), out = o in fp32, out_bf = o in bf16
+ * (either may be NULL; without both, pre_weight may be NULL).  The norm
+ * weights are bf16 [hidden].  hidden % 4 == 0, <= 32768; fp32 rows 16-byte,
+ * bf16 rows 8-byte aligned.
+ *   grimoire_block_norm: f = x[t], fp32 or (x_bf16) bf16 rows x_stride
+ *     elements apart (a multiple of 4, >= hidden).
+ *   grimoire_moe_block_norm: f = shared[t] (fp32, may be NULL) + sum_s
+ *     route_weight[t,s] * routed[inverse[t,s]], an fma chain in slot order;
+ *     routed bf16 [routed_rows][hidden];
+ *     a slot whose inverse lies outside [0, routed_rows) is skipped;
+ *     top_k <= 16: the combine of grimoire_moe_rmsnorm_residual. */
+enum grim_gate_kind {
+    GRIM_GATE_NONE = 0,
+    GRIM_GATE_CHANNEL = 1,
+    GRIM_GATE_ROW = 2,
+    GRIM_GATE_FULL = 3
+};
+typedef struct grim_block_norm_params {
+    const uint16_t* post_weight;
+    const uint16_t* pre_weight;
+    float weight_offset;
+    float eps;
+    float residual_scale;
+    float block_scale;
+    int32_t gate_kind;         /* enum grim_gate_kind                      */
+    int32_t gate_sigmoid;
+} grim_block_norm_params;
+int grimoire_block_norm(void* stream, const grim_block_norm_params* p, const void* gate,
+                        int gate_bf16, const float* h, const void* x, int x_bf16, int64_t x_stride,
+                        float* h_out, float* out, uint16_t* out_bf, int tokens, int hidden);
+int grimoire_moe_block_norm(void* stream, const grim_block_norm_params* p, const void* gate,
+                            int gate_bf16, const float* h, const uint16_t* routed, int routed_rows,
+                            const int32_t* inverse, const float* route_weight, const float* shared,
+                            float* h_out, float* out, uint16_t* out_bf, int tokens, int top_k,
+                            int hidden);
 
 /* ------------------------------------------------------------------------
  * Expert-weight ingestion: one checkpoint projection [out][in] of one expert

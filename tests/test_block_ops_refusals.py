@@ -1,0 +1,83 @@
+"""Host-side refusals of the block operators' entry points: nothing here
+reaches a kernel (the pointers are not memory)."""
+import ctypes as C
+
+import pytest
+import torch
+
+from grimoire_amd import _abi, ops
+
+OK, SHAPE, ARG = 0, _abi.ERR_SHAPE, _abi.ERR_ARG
+A = 1 << 12   # an aligned address nothing is read from
+
+
+def scores(n_experts=64, top_k=8, row_stride=None, logits=A, ids=A, w=A, tokens=2, null=False, **kw):
+    p = _abi.ScoreParams(score=0, n_group=1, topk_group=1, group_score=0, normalize=1, scaling=1.0)
+    for k, v in kw.items():
+        setattr(p, k, v)
+    return _abi.lib().grimoire_moe_router_scores(None, None if null else C.byref(p), logits, 0,
+                                                 n_experts if row_stride is None else row_stride, tokens, n_experts,
+                                                 top_k, ids, w)
+
+
+@pytest.mark.parametrize("kw,status", [
+    (dict(tokens=0), OK), (dict(tokens=0, logits=None), OK), (dict(tokens=-1), OK),
+    (dict(logits=None), ARG), (dict(ids=None), ARG), (dict(w=None), ARG), (dict(null=True), ARG), (dict(score=2), ARG),
+    (dict(n_experts=0, row_stride=1), SHAPE), (dict(n_experts=513), SHAPE), (dict(top_k=0), SHAPE),
+    (dict(top_k=17), SHAPE), (dict(n_experts=4, top_k=5), SHAPE), (dict(row_stride=63), SHAPE),
+    (dict(n_group=-1), SHAPE), (dict(n_group=7, topk_group=1), SHAPE), (dict(n_group=8, topk_group=0), SHAPE),
+    (dict(n_group=8, topk_group=9), SHAPE), (dict(n_group=16, topk_group=1), SHAPE),
+    (dict(n_group=8, topk_group=1, group_score=2), ARG),
+    (dict(n_experts=130, n_group=65, topk_group=65, top_k=1), SHAPE)])
+def test_scores(kw, status):
+    assert scores(**kw) == status
+
+
+def norm(h=A, x=A, h_out=A, out=A, out_bf=None, tokens=2, hidden=64, x_stride=None, gate=None, gate_bf16=0, x_bf16=0,
+         **kw):
+    p = _abi.BlockNormParams(post_weight=A, pre_weight=A, weight_offset=1.0, eps=1e-6, residual_scale=1.0,
+                             block_scale=1.0, gate_kind=0, gate_sigmoid=0)
+    for k, v in kw.items():
+        setattr(p, k, v)
+    return _abi.lib().grimoire_block_norm(None, C.byref(p), gate, gate_bf16, h, x, x_bf16,
+                                          hidden if x_stride is None else x_stride, h_out, out, out_bf, tokens, hidden)
+
+
+def moe_norm(routed=A, rows=9, inverse=A, rw=A, shared=None, top_k=4, hidden=64, tokens=2):
+    p = _abi.BlockNormParams(post_weight=A, pre_weight=A, weight_offset=1.0, eps=1e-6, residual_scale=1.0,
+                             block_scale=1.0, gate_kind=0, gate_sigmoid=0)
+    return _abi.lib().grimoire_moe_block_norm(None, C.byref(p), None, 0, A, routed, rows, inverse, rw, shared, A, A,
+                                              None, tokens, top_k, hidden)
+
+
+@pytest.mark.parametrize("kw,status", [
+    (dict(tokens=0), OK), (dict(tokens=0, h=None), OK), (dict(h=None), ARG), (dict(x=None), ARG),
+    (dict(hidden=66), SHAPE), (dict(hidden=0), SHAPE), (dict(hidden=32772), SHAPE), (dict(x_stride=60), SHAPE),
+    (dict(x_stride=66), SHAPE), (dict(h_out=None, out=None), ARG), (dict(pre_weight=None), ARG),
+    (dict(gate_kind=4, gate=A), ARG), (dict(gate_kind=1), ARG), (dict(gate=A), ARG), (dict(h=A + 4), ARG),
+    (dict(x=A + 8), ARG), (dict(x=A + 4, x_bf16=1), ARG), (dict(out=A + 8), ARG), (dict(out_bf=A + 4), ARG),
+    (dict(h_out=A + 4), ARG), (dict(post_weight=A + 4), ARG), (dict(gate_kind=1, gate=A + 8), ARG),
+    (dict(gate_kind=3, gate=A + 4, gate_bf16=1), ARG), (dict(gate_kind=2, gate=A + 2), ARG)])
+def test_block_norm(kw, status):
+    assert norm(**kw) == status
+
+
+@pytest.mark.parametrize("kw,status", [
+    (dict(tokens=0), OK), (dict(routed=None), ARG), (dict(inverse=None), ARG), (dict(rw=None), ARG),
+    (dict(top_k=0), SHAPE), (dict(top_k=17), SHAPE), (dict(rows=-1), SHAPE), (dict(hidden=2), SHAPE),
+    (dict(routed=A + 4), ARG), (dict(shared=A + 4), ARG)])
+def test_moe_block_norm(kw, status):
+    assert moe_norm(**kw) == status
+
+
+def test_cpu_tensors_and_bad_names():
+    with pytest.raises(_abi.GrimoireError):
+        ops.RouteScores()(torch.zeros(2, 8), torch.zeros(2, 2, dtype=torch.int32), torch.zeros(2, 2))
+    with pytest.raises(_abi.GrimoireError):
+        ops.RouteScores(score="relu")
+    with pytest.raises(_abi.GrimoireError):
+        ops.RouteScores(bias=torch.zeros(8))
+    with pytest.raises(_abi.GrimoireError):
+        ops.BlockNorm(None)(torch.zeros(2, 8), torch.zeros(2, 8), torch.zeros(2, 8))
+    with pytest.raises(_abi.GrimoireError):
+        ops.BlockNorm(None, gate="head")
