@@ -136,6 +136,13 @@ class BlockNormParams(C.Structure):
 
 GATE_NONE, GATE_CHANNEL, GATE_ROW, GATE_FULL = 0, 1, 2, 3
 
+
+class Lora(C.Structure):
+    """grim_lora"""
+    _fields_ = [("K", C.c_int32), ("N", C.c_int32), ("slots", C.c_int32), ("max_rank", C.c_int32),
+                ("a", C.c_void_p), ("b", C.c_void_p), ("rank", C.c_void_p), ("scale", C.c_void_p)]
+
+
 P = C.c_void_p
 I32 = C.c_int
 F32 = C.c_float
@@ -181,6 +188,9 @@ SIGNATURES = {
     "grimoire_block_norm": (I32, [P, C.POINTER(BlockNormParams), P, I32, P, P, I32, I64, P, P, P, I32, I32]),
     "grimoire_moe_block_norm": (I32, [P, C.POINTER(BlockNormParams), P, I32, P, P, I32, P, P, P, P, P, P, I32,
                                       I32, I32]),
+    "grimoire_lora_workspace_bytes": (SZ, [C.POINTER(Lora), I32]),
+    "grimoire_lora_add": (I32, [P, C.POINTER(Lora), P, P, I32, I64, P, I32, I64, P, I32, I64, I32, P, SZ]),
+    "grimoire_lora_swiglu": (I32, [P, C.POINTER(Lora), P, P, I32, I64, P, I32, I64, P, I32, I64, I32, P, SZ]),
     "grimoire_moe_ingest_projection": (I32, [P, C.POINTER(ExpertSrc), QWP, I32]),
     "grimoire_moe_ingest_projections": (I32, [P, C.POINTER(ExpertSrc), P, I32, QWP]),
     "grimoire_moe_int4_to_signed": (I32, [P, P, SZ, P, SZ, P, SZ, P, SZ, P]),

@@ -21,6 +21,7 @@
 #include "gemv.hpp"
 #include "elementwise.hpp"
 #include "ingest.hpp"
+#include "lora.hpp"
 #include "tiered.hpp"
 #include "router.hpp"
 #include "scores.hpp"
@@ -527,6 +528,57 @@ int grimoire_moe_block_norm(void* stream, const grim_block_norm_params* p, const
     if (!aligned(routed, 8) || !aligned(shared, 16)) return fail(GRIM_ERR_ARG, "routed/shared alignment");
     a.routed = routed; a.routed_rows = routed_rows; a.inverse = inverse; a.rw = route_weight; a.shared = shared; a.K = top_k;
     return status(block_norm_launch(S(stream), a));
+}
+
+size_t grimoire_lora_workspace_bytes(const grim_lora* L, int rows) {
+    return L ? lora_workspace_bytes(L->K, L->max_rank, rows) : 0;
+}
+
+static int lora_common(void* stream, const grim_lora* L, const int32_t* row_slot, const void* x, int x_bf16,
+                       int64_t x_stride, const void* base, int base_bf16, int64_t base_stride, void* y,
+                       int y_bf16, int64_t y_stride, int rows, void* ws, size_t ws_bytes, int glu) {
+    if (rows <= 0) return GRIM_OK;
+    if (!L || !L->a || !L->b || !L->rank || !L->scale || !row_slot || !x || !base || !y)
+        return fail(GRIM_ERR_ARG, "null pointer");
+    if (L->K <= 0 || L->K % 8) return fail(GRIM_ERR_SHAPE, "K=%d (need %% 8)", L->K);
+    if (L->N <= 0 || L->N % (glu ? 8 : 4)) return fail(GRIM_ERR_SHAPE, "N=%d (need %% %d)", L->N, glu ? 8 : 4);
+    if (L->slots <= 0) return fail(GRIM_ERR_SHAPE, "slots=%d", L->slots);
+    if (L->max_rank <= 0 || L->max_rank % 16 || L->max_rank > kLoraMaxRank)
+        return fail(GRIM_ERR_SHAPE, "max_rank=%d (a multiple of 16, <= %d)", L->max_rank, kLoraMaxRank);
+    const int width = glu ? L->N / 2 : L->N;
+    if (x_stride < L->K || x_stride % 8) return fail(GRIM_ERR_SHAPE, "x_stride=%lld", (long long)x_stride);
+    if (base_stride < L->N || base_stride % 4) return fail(GRIM_ERR_SHAPE, "base_stride=%lld", (long long)base_stride);
+    if (y_stride < width || y_stride % 4) return fail(GRIM_ERR_SHAPE, "y_stride=%lld", (long long)y_stride);
+    if (!aligned(L->a, 16) || !aligned(L->b, 16) || !aligned(x, 16) || !aligned(base, base_bf16 ? 8 : 16) ||
+        !aligned(y, y_bf16 ? 8 : 16))
+        return fail(GRIM_ERR_ARG, "adapters, x and fp32 rows 16-byte, bf16 rows 8-byte alignment");
+    if (y == base && (glu || !base_bf16 != !y_bf16 || base_stride != y_stride))
+        return fail(GRIM_ERR_ARG, "in place needs the same type and stride (and no SwiGLU)");
+    const size_t need = lora_workspace_bytes(L->K, L->max_rank, rows);
+    if (!ws || ws_bytes < need) return fail(GRIM_ERR_WORKSPACE, "adapter workspace too small (need %zu)", need);
+    if (!aligned(ws, 16)) return fail(GRIM_ERR_ARG, "workspace not 16-byte aligned");
+    LoraArgs a{};
+    a.a = L->a; a.b = L->b; a.rank = L->rank; a.scale = L->scale;
+    a.slots = L->slots; a.R = L->max_rank; a.K = L->K; a.N = L->N;
+    a.row_slot = row_slot; a.x = x; a.base = base; a.y = y;
+    a.x_stride = x_stride; a.base_stride = base_stride; a.y_stride = y_stride;
+    a.x_bf16 = x_bf16 ? 1 : 0; a.base_bf16 = base_bf16 ? 1 : 0; a.y_bf16 = y_bf16 ? 1 : 0;
+    a.T = rows; a.glu = glu; a.part = static_cast<float*>(ws);
+    return status(lora_launch(S(stream), a));
+}
+
+int grimoire_lora_add(void* stream, const grim_lora* L, const int32_t* row_slot, const void* x, int x_bf16,
+                      int64_t x_stride, const void* base, int base_bf16, int64_t base_stride, void* y,
+                      int y_bf16, int64_t y_stride, int rows, void* workspace, size_t workspace_bytes) {
+    return lora_common(stream, L, row_slot, x, x_bf16, x_stride, base, base_bf16, base_stride, y, y_bf16,
+                       y_stride, rows, workspace, workspace_bytes, 0);
+}
+
+int grimoire_lora_swiglu(void* stream, const grim_lora* L, const int32_t* row_slot, const void* x, int x_bf16,
+                         int64_t x_stride, const void* base, int base_bf16, int64_t base_stride, void* h,
+                         int h_bf16, int64_t h_stride, int rows, void* workspace, size_t workspace_bytes) {
+    return lora_common(stream, L, row_slot, x, x_bf16, x_stride, base, base_bf16, base_stride, h, h_bf16,
+                       h_stride, rows, workspace, workspace_bytes, 1);
 }
 
 static int ingest_common(void* stream, const grim_expert_src* srcs, const int32_t* row0s, int n,

@@ -15,7 +15,7 @@ import torch
 
 from . import _abi
 from ._abi import check, lib
-from .weights import MoeLayer, Weight
+from .weights import LoraAdapters, MoeLayer, Weight
 
 
 def _p(t: Optional[torch.Tensor]):
@@ -460,6 +460,49 @@ class BlockNorm:
                 _flat(inverse.view(-1), "inverse", (T * K,), _I32, dev),
                 _flat(route_weight, "route_weight", (T, K), _F32, dev), _flat(shared, "shared", (T, H), _F32, dev), hop,
                 op, obp, T, K, H)
+
+
+# ------------------------------------------------------ low-rank adapters
+
+class Lora:
+    """Low-rank adapters of many requests beside one shared projection
+    (grimoire_lora_add / grimoire_lora_swiglu), with the workspace of up to
+    max_rows rows."""
+
+    def __init__(self, adapters: LoraAdapters, max_rows: int):
+        _dev(adapters.a)
+        self.adapters = adapters
+        self.struct = adapters.struct()
+        self.max_rows = max_rows
+        self.dev = adapters.a.get_device()
+        nbytes = int(lib().grimoire_lora_workspace_bytes(self.struct, max_rows))
+        self.workspace = torch.empty(nbytes, dtype=torch.uint8, device=adapters.a.device)
+
+    def _call(self, fn, what, row_slot, x, base, y, width, stream):
+        _dev(x)
+        A, dev = self.adapters, self.dev
+        T = x.shape[0]
+        if T > self.max_rows:
+            raise _abi.GrimoireError("more rows than the workspace was sized for")
+        if x.get_device() != dev or base.get_device() != dev or y.get_device() != dev:
+            raise _abi.GrimoireError(f"{what}: x, base, output and adapters on different devices")
+        xp, x16, xs = _rows(x, "x", A.K, T)
+        bp, b16, bs = _rows(base, "base", A.N, T)
+        yp, y16, ys = _rows(y, "output", width, T)
+        _launch(x, stream, fn, what, self.struct, _flat(row_slot, "row_slot", (T,), _I32, dev), xp, x16, xs, bp, b16,
+                bs, yp, y16, ys, T, self.workspace.data_ptr(), self.workspace.numel())
+
+    def add(self, row_slot, x, y, base=None, stream=None):
+        """y = base + the adapters' product of x (base None: y += it).
+        row_slot int32 [T]; x [T][K], base and y [T][N] fp32 or bf16, rows
+        may lie apart."""
+        self._call(lib().grimoire_lora_add, "lora_add", row_slot, x, y if base is None else base, y, self.adapters.N,
+                   stream)
+
+    def swiglu(self, row_slot, x, base, h, stream=None):
+        """h [T][N/2] = silu(gate) * up of the gate|up projection base
+        [T][N] plus the adapters' product of x."""
+        self._call(lib().grimoire_lora_swiglu, "lora_swiglu", row_slot, x, base, h, self.adapters.N // 2, stream)
 
 
 # ------------------------------------------------------------------- layer

@@ -215,3 +215,50 @@ class MoeLayer:
         if not self.has_shared:
             return 0.0
         return float(self.shared_gate_up.nbytes() + self.shared_down.nbytes())
+
+
+@dataclass
+class LoraAdapters:
+    """The low-rank adapters of one projection [N][K], in slots
+    (grim_lora): a [slots][max_rank][K] and b [slots][N][max_rank] bf16 (or
+    their bits as int16), rank int32 [slots], scale fp32 [slots], all on one
+    device.  What a slot holds past its rank is not part of its adapter."""
+    a: torch.Tensor
+    b: torch.Tensor
+    rank: torch.Tensor
+    scale: torch.Tensor
+
+    def __post_init__(self):
+        S, R, K = self.a.shape
+        N = self.b.shape[1]
+        for t, shape, types in ((self.a, (S, R, K), (torch.bfloat16, torch.int16)),
+                                (self.b, (S, N, R), (torch.bfloat16, torch.int16)),
+                                (self.rank, (S,), (torch.int32,)), (self.scale, (S,), (torch.float32,))):
+            if t.shape != shape or t.dtype not in types or not t.is_contiguous() or t.device != self.a.device:
+                raise _abi.GrimoireError(f"adapters: {t.dtype} {tuple(t.shape)} on {t.device}, expected "
+                                         f"contiguous {shape} on {self.a.device}")
+        self.slots, self.max_rank, self.K, self.N = S, R, K, N
+
+    @staticmethod
+    def empty(slots: int, max_rank: int, K: int, N: int, device="cuda") -> "LoraAdapters":
+        """Free slots: every rank 0."""
+        return LoraAdapters(torch.zeros((slots, max_rank, K), dtype=torch.bfloat16, device=device),
+                            torch.zeros((slots, N, max_rank), dtype=torch.bfloat16, device=device),
+                            torch.zeros((slots,), dtype=torch.int32, device=device),
+                            torch.zeros((slots,), dtype=torch.float32, device=device))
+
+    def load(self, slot: int, a: torch.Tensor, b: torch.Tensor, scale: float) -> None:
+        """An adapter's A [r][K] and B [N][r] into a slot (r <= max_rank;
+        rounded to bf16 when they are not), in the current stream's order."""
+        r = a.shape[0]
+        if not 0 <= slot < self.slots or r > self.max_rank or a.shape != (r, self.K) or b.shape != (self.N, r):
+            raise _abi.GrimoireError(f"slot {slot}: A {tuple(a.shape)}, B {tuple(b.shape)} for "
+                                     f"[{self.N}][{self.K}] of rank <= {self.max_rank}")
+        self.a.view(torch.bfloat16)[slot, :r].copy_(a)
+        self.b.view(torch.bfloat16)[slot, :, :r].copy_(b)
+        self.rank[slot] = r
+        self.scale[slot] = scale
+
+    def struct(self) -> _abi.Lora:
+        return _abi.Lora(self.K, self.N, self.slots, self.max_rank, self.a.data_ptr(), self.b.data_ptr(),
+                         self.rank.data_ptr(), self.scale.data_ptr())

@@ -402,6 +402,48 @@ int grimoire_moe_block_norm(void* stream, const grim_block_norm_params* p, const
                             int hidden);
 
 /* ------------------------------------------------------------------------
+ * Low-rank adapters of many requests beside a projection they share (no
+ * counterpart in the reference).  Adapter a of the projection [N][K] is
+ * scale_a B_a A_a, A_a [rank_a][K], B_a [N][rank_a]; it lives in a slot of
+ * two stacked bf16 tensors, of which only the first rank_a rows of A and
+ * columns of B are part of it (the rest is not used, whatever it holds).
+ * Row t of a batch uses the adapter in slot row_slot[t]; a row whose slot
+ * lies outside [0, slots) has none.
+ * ---------------------------------------------------------------------- */
+typedef struct grim_lora {
+    int32_t K;                 /* input features, a multiple of 8          */
+    int32_t N;                 /* output features, a multiple of 4         */
+    int32_t slots;
+    int32_t max_rank;          /* a multiple of 16, <= 256                 */
+    const uint16_t* a;         /* bf16 [slots][max_rank][K]                */
+    const uint16_t* b;         /* bf16 [slots][N][max_rank]                */
+    const int32_t* rank;       /* device [slots], taken into [0, max_rank] */
+    const float* scale;        /* device [slots]                           */
+} grim_lora;
+
+/* Device workspace of the calls below for up to `rows` rows (16-byte
+ * aligned, no initial contents needed).  Calls that share one must not
+ * overlap: two graphs that hold it run one after the other. */
+size_t grimoire_lora_workspace_bytes(const grim_lora* L, int rows);
+/* y[t] = base[t] + scale_a B_a (A_a x[t]); rows without an adapter are
+ * copied (in place: left as they are).  x [rows][K], base and y [rows][N]:
+ * fp32 or bf16 rows, *_stride elements apart (x a multiple of 8, base and y
+ * of 4); fp32 and x rows 16-byte, bf16 base and y rows 8-byte aligned.  y may
+ * be base (same type and stride) and overlaps nothing else.  Sums are fp32,
+ * in an order that does not depend on the other rows' adapters; fp32
+ * activations are multiplied in full precision. */
+int grimoire_lora_add(void* stream, const grim_lora* L, const int32_t* row_slot, const void* x, int x_bf16,
+                      int64_t x_stride, const void* base, int base_bf16, int64_t base_stride, void* y,
+                      int y_bf16, int64_t y_stride, int rows, void* workspace, size_t workspace_bytes);
+/* The same on a gate|up projection (N = 2I, gate columns first; I a multiple
+ * of 4) with the SwiGLU behind it: v = base[t] + scale_a B_a (A_a x[t]),
+ * h[t][i] = silu(v[i]) * v[I + i].  base [rows][2I], h [rows][I] (apart). */
+int grimoire_lora_swiglu(void* stream, const grim_lora* L, const int32_t* row_slot, const void* x,
+                         int x_bf16, int64_t x_stride, const void* base, int base_bf16,
+                         int64_t base_stride, void* h, int h_bf16, int64_t h_stride, int rows,
+                         void* workspace, size_t workspace_bytes);
+
+/* ------------------------------------------------------------------------
  * Expert-weight ingestion: one checkpoint projection [out][in] of one expert
  * into rows [row0, row0 + out) of a stacked weight, the per-expert staging
  * of src/grimoire.cpp:8340-8383 (gate at expert*2I, up at expert*2I + I in

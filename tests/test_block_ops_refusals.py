@@ -5,7 +5,7 @@ import ctypes as C
 import pytest
 import torch
 
-from grimoire_amd import _abi, ops
+from grimoire_amd import _abi, ops, weights
 
 OK, SHAPE, ARG = 0, _abi.ERR_SHAPE, _abi.ERR_ARG
 A = 1 << 12   # an aligned address nothing is read from
@@ -68,6 +68,59 @@ def test_block_norm(kw, status):
     (dict(routed=A + 4), ARG), (dict(shared=A + 4), ARG)])
 def test_moe_block_norm(kw, status):
     assert moe_norm(**kw) == status
+
+
+def lora(glu=False, rows=3, slot=A, x=A, x_bf16=0, x_stride=64, base=A, base_bf16=0, base_stride=32, y=2 * A, y_bf16=0,
+         y_stride=None, ws=A, ws_bytes=1 << 20, **kw):
+    L = _abi.Lora(K=64, N=32, slots=4, max_rank=16, a=A, b=A, rank=A, scale=A)
+    for k, v in kw.items():
+        setattr(L, k, v)
+    fn = _abi.lib().grimoire_lora_swiglu if glu else _abi.lib().grimoire_lora_add
+    return fn(None, C.byref(L), slot, x, x_bf16, x_stride, base, base_bf16, base_stride, y, y_bf16,
+              (16 if glu else 32) if y_stride is None else y_stride, rows, ws, ws_bytes)
+
+
+@pytest.mark.parametrize("kw,status", [
+    (dict(rows=0), OK), (dict(rows=0, x=None), OK), (dict(slot=None), ARG), (dict(x=None), ARG), (dict(base=None), ARG),
+    (dict(y=None), ARG), (dict(a=None), ARG), (dict(b=None), ARG), (dict(rank=None), ARG), (dict(scale=None), ARG),
+    (dict(K=0), SHAPE), (dict(K=60), SHAPE), (dict(N=30), SHAPE), (dict(N=0), SHAPE), (dict(slots=0), SHAPE),
+    (dict(max_rank=0), SHAPE), (dict(max_rank=24), SHAPE), (dict(max_rank=272), SHAPE), (dict(x_stride=56), SHAPE),
+    (dict(x_stride=68), SHAPE), (dict(base_stride=28), SHAPE), (dict(base_stride=34), SHAPE),
+    (dict(y_stride=28), SHAPE), (dict(y_stride=33), SHAPE), (dict(x=A + 8), ARG), (dict(base=A + 8), ARG),
+    (dict(base=A + 4, base_bf16=1), ARG), (dict(y=A + 8), ARG), (dict(a=A + 8), ARG), (dict(b=A + 2), ARG),
+    (dict(y=A, y_bf16=1), ARG), (dict(y=A, y_stride=36), ARG), (dict(glu=True, y=A), ARG),
+    (dict(glu=True, N=36, base_stride=36), SHAPE), (dict(glu=True, y_stride=12), SHAPE),
+    (dict(ws=None), _abi.ERR_WORKSPACE), (dict(ws_bytes=3 * 16 * 4 - 1), _abi.ERR_WORKSPACE), (dict(ws=A + 4), ARG)])
+def test_lora(kw, status):
+    assert lora(**kw) == status
+
+
+def test_lora_workspace_grows_with_rows():
+    """One size holds every shorter batch, those that split K among them."""
+    for K in (8, 64, 2048, 7168):
+        L = _abi.Lora(K=K, N=32, slots=4, max_rank=32)
+        n = [_abi.lib().grimoire_lora_workspace_bytes(C.byref(L), r) for r in (1, 16, 511, 512, 513, 700, 5000, 9000)]
+        assert n == sorted(n) and n[0] >= 32 * 4
+    assert _abi.lib().grimoire_lora_workspace_bytes(None, 5) == 0
+    assert _abi.lib().grimoire_lora_workspace_bytes(C.byref(L), 0) == 0
+
+
+def test_lora_adapters_shapes():
+    ad = weights.LoraAdapters.empty(3, 16, 64, 32, device="cpu")
+    ad.load(1, torch.ones(5, 64), torch.ones(32, 5), 0.5)
+    assert ad.rank.tolist() == [0, 5, 0] and float(ad.a.sum()) == 5 * 64 and float(ad.b[1, :, 5:].sum()) == 0
+    for bad in (dict(slot=3), dict(slot=-1), dict(a=torch.ones(17, 64), b=torch.ones(32, 17)),
+                dict(a=torch.ones(5, 63)), dict(b=torch.ones(32, 6))):
+        kw = dict(slot=0, a=torch.ones(5, 64), b=torch.ones(32, 5), scale=1.0)
+        kw.update(bad)
+        with pytest.raises(_abi.GrimoireError):
+            ad.load(**kw)
+    with pytest.raises(_abi.GrimoireError):
+        weights.LoraAdapters(ad.a, ad.b[:, :, :8], ad.rank, ad.scale)
+    with pytest.raises(_abi.GrimoireError):
+        weights.LoraAdapters(ad.a.float(), ad.b, ad.rank, ad.scale)
+    with pytest.raises(_abi.GrimoireError):
+        ops.Lora(ad, 4)
 
 
 def test_cpu_tensors_and_bad_names():
