@@ -21,6 +21,7 @@ FMT_INT4_F16 = 64
 ROUTE_SOFTMAX = 0
 ROUTE_SIGMOID = 1
 ROUTE_GROUP = 2
+ROUTE_PROBS = 3
 
 
 ERR_FORMAT, ERR_SHAPE, ERR_ARG, ERR_WORKSPACE = -1, -2, -3, -4

@@ -27,6 +27,7 @@
 #include "gemv_mx.hpp"
 #include "gemv.hpp"
 #include "router.hpp"
+#include "scores.hpp"
 
 using namespace grim;
 
@@ -803,6 +804,12 @@ static int forward_impl(void* stream, const grim_moe_layer* L, const grim_route_
     const auto& c = L->cfg;
     if (L->has_shared && c.shared_inter != c.inter)
         return ferr(GRIM_ERR_SHAPE, "shared_inter must equal inter");
+    // probabilities over all experts: the router scores kernel routes, a
+    // launch of its own (the decode kernels' own top-k weighs the picks alone)
+    const bool probs = rp && rp->mode == GRIM_ROUTE_PROBS;
+    if (probs && roles != (kRoleRouter | kRoleGateUp | kRoleDown))
+        return ferr(GRIM_ERR_ARG, "decode stages do not take GRIM_ROUTE_PROBS");
+    if (probs && (regime == 1 || regime == 7)) regime = 3;
     const PlanKind kind = plan_kind(L, tokens, regime, workspace_bytes, shard_count);
     const bool gemv = kind == PlanKind::kSlots;
     Plan p{};
@@ -820,8 +827,10 @@ static int forward_impl(void* stream, const grim_moe_layer* L, const grim_route_
         return ferr(GRIM_ERR_ARG, "expert shard outside [0, num_experts)");
     const int mode = rp ? rp->mode : GRIM_ROUTE_SOFTMAX;
     if (H % 4) return ferr(GRIM_ERR_SHAPE, "hidden must be a multiple of 4");
-    if (mode < GRIM_ROUTE_SOFTMAX || mode > GRIM_ROUTE_GROUP) return ferr(GRIM_ERR_ARG, "unknown route mode");
-    if (mode == GRIM_ROUTE_GROUP &&
+    if (mode < GRIM_ROUTE_SOFTMAX || mode > GRIM_ROUTE_PROBS) return ferr(GRIM_ERR_ARG, "unknown route mode");
+    const bool grouped = mode == GRIM_ROUTE_GROUP || (probs && rp->n_group > 1);
+    if (probs && rp->n_group < 0) return ferr(GRIM_ERR_SHAPE, "group-limited routing parameters");
+    if (grouped &&
         (!rp || rp->n_group <= 0 || rp->n_group > 64 || E % rp->n_group || rp->topk_group <= 0 ||
          rp->topk_group > rp->n_group || K > rp->topk_group * (E / rp->n_group)))
         return ferr(GRIM_ERR_SHAPE, "group-limited routing parameters");
@@ -833,7 +842,7 @@ static int forward_impl(void* stream, const grim_moe_layer* L, const grim_route_
     const float scaling = (rp && mode != GRIM_ROUTE_SOFTMAX) ? rp->scaling : 1.0f;
     const bool sh = L->has_shared;
 
-    const bool decode = gemv && regime != 3 && tokens <= kDecodeMaxTokens && !shard;
+    const bool decode = gemv && regime != 3 && tokens <= kDecodeMaxTokens && !shard && !probs;
     if (gemv && !decode) {
         // what the slot kernels' entry points check (of a shard, its own
         // experts), before anything is launched
@@ -930,14 +939,14 @@ static int forward_impl(void* stream, const grim_moe_layer* L, const grim_route_
                     (regime == 4 || regime == 5 || (regime == 0 && int64_t(tokens) * K <= 2 * int64_t(E))) &&
                     !(regime == 5 && layer_mx_padded(L));   // the vector-ALU one reads packed rows only
     const bool gv_mx = gv && regime != 5 && L->gate_up.fmt == GRIM_FMT_MXFP4 && gvm_shape_ok(H, I);
-    if (gv_mx && int64_t(tokens) * K <= kGvmRouteMax && !shard) {
+    if (gv_mx && int64_t(tokens) * K <= kGvmRouteMax && !shard && !probs) {
         if (deferred) {
             hipError_t e = router_finish_launch(st, p.logits, p.logits2, rbias, tokens, E);
             if (e != hipSuccess) return ferr(int(e), hipGetErrorString(e));
         }
         return forward_gv(st, L, p, x, y, tokens, shared_gate_w, true, &tka);
     }
-    if (kind == PlanKind::kWreg && !shard && !deferred && wreg_one_dispatch(tokens, K, E) && wreg_one_topk(tokens))
+    if (kind == PlanKind::kWreg && !shard && !probs && !deferred && wreg_one_dispatch(tokens, K, E) && wreg_one_topk(tokens))
         return forward_wreg(st, L, p, x, y, tokens, shared_gate_w, &tka);
     if (deferred) {
         // the top-k finishes the split router's sum as it loads
@@ -945,7 +954,10 @@ static int forward_impl(void* stream, const grim_moe_layer* L, const grim_route_
         tka.lbias = rbias;
     }
     {
-        hipError_t e = topk_launch(st, tka);
+        ScoresArgs sa{p.logits, E, 0, tokens, E, K, 0, probs ? static_cast<const float*>(rp->bias) : nullptr,
+                      probs && rp->n_group > 1 ? rp->n_group : 1, probs ? rp->topk_group : 1, 0, c.norm_topk,
+                      scaling, p.rex, p.rwt, tka.part1, nullptr};
+        hipError_t e = probs ? scores_launch(st, sa) : topk_launch(st, tka);
         if (e != hipSuccess) return ferr(int(e), hipGetErrorString(e));
     }
     // one expert shard: the routes it owns become local indices, the rest

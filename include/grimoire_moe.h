@@ -806,18 +806,22 @@ void grimoire_xe2_fused_moe_gate_up_mxfp4_silu_bf16(void* stream, const void* ac
 enum grim_route_mode {
     GRIM_ROUTE_SOFTMAX = 0,    /* softmax top-k (+ renormalise per cfg)   */
     GRIM_ROUTE_SIGMOID = 1,    /* sigmoid + selection bias (bf16)         */
-    GRIM_ROUTE_GROUP = 2       /* group-limited sigmoid (bias fp32)       */
+    GRIM_ROUTE_GROUP = 2,      /* group-limited sigmoid (bias fp32)       */
+    GRIM_ROUTE_PROBS = 3       /* probabilities of a softmax over all
+                                  experts (grimoire_moe_router_scores with
+                                  GRIM_SCORE_SOFTMAX and GRIM_GROUP_MAX);
+                                  no reference counterpart                */
 };
 
 typedef struct grim_route_params {
     int32_t mode;              /* enum grim_route_mode                     */
-    int32_t n_group;           /* GROUP only                               */
-    int32_t topk_group;        /* GROUP only                               */
+    int32_t n_group;           /* GROUP; PROBS: 1 or 0 = no group limit    */
+    int32_t topk_group;        /* GROUP, and PROBS with n_group > 1        */
     float scaling;             /* routed scaling factor (1 = none)         */
     const void* bias;          /* SOFTMAX: router bias fp32 [E] added to the
                                   logits (logits = W x + b); SIGMOID: bf16
-                                  [E] selection bias; GROUP: fp32 [E]
-                                  selection bias; or NULL */
+                                  [E] selection bias; GROUP, PROBS: fp32
+                                  [E] selection bias; or NULL */
 } grim_route_params;
 
 /* Workspace bytes for grimoire_moe_forward at `tokens`.  Its first
@@ -851,7 +855,8 @@ size_t grimoire_moe_forward_workspace_bytes(const grim_moe_layer* L, int tokens)
  * grimoire_moe_decode_sync_status reports it), 4 = expert-grouped
  * GEMV (MXFP4 with hidden and inter multiples of 64 above 256: on the
  * scaled fp4 matrix core, K padded to 256; otherwise on the vector ALU), 5 = expert-grouped GEMV on
- * the vector ALU.  No reference counterpart for 3-5 (regimes of this
+ * the vector ALU.  GRIM_ROUTE_PROBS routes in a launch of its own: regimes 1
+ * and 7 run as 3.  No reference counterpart for 3-5 (regimes of this
  * build; the reference picks its kernels per batch size the same way). */
 int grimoire_moe_forward(void* stream, const grim_moe_layer* L, const grim_route_params* rp,
                          const uint16_t* shared_gate_w, const float* x, float* y, int tokens,
