@@ -12,10 +12,15 @@
 // order of the sum, about once in 10^5 picks at E = 512; in fp64 the choice
 // is that of the exact scores.  It costs E exps of the fp64 pipe a token.
 //
-// Lanes: each group owns lpg = 2^floor(log2(64 / n_group)) lanes of V =
-// ceil(group / lpg) <= 16 consecutive experts, so a group's reductions are
-// butterflies inside its lanes and the lowest lane (then its lowest slot)
-// holding a value is the lowest expert.
+// Lanes: without groups expert e is lane e % 64's, so a load of a lane's j-th
+// expert is one run of memory.  With groups each owns lpg =
+// 2^floor(log2(64 / n_group)) lanes of V = ceil(group / lpg) <= 16
+// consecutive experts: a group's reductions are butterflies in its lanes.
+//
+// The choice: K rounds over the lanes' best values, rounded to fp32, give a
+// bound that at least K experts reach (rounding keeps the order); the few
+// experts that reach it are gathered, one a lane, and ranked against each
+// other in fp64.  More than 64 of them (ties) take K rounds over all values.
 #include "scores.hpp"
 #include "topk.hpp"
 
@@ -31,10 +36,50 @@ __device__ __forceinline__ double shfl_xor_d(double v, int o) {
     return __hiloint2double(hi, lo);
 }
 
+__device__ __forceinline__ double lane_d(double v, int lane) {
+    return __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(v), lane),
+                            __builtin_amdgcn_readlane(__double2loint(v), lane));
+}
+
+template <int CTRL>
+__device__ __forceinline__ double dpp_d(double v) {
+    return __hiloint2double(int(dpp_u<CTRL>(uint32_t(__double2hiint(v)))),
+                            int(dpp_u<CTRL>(uint32_t(__double2loint(v)))));
+}
+
+// Sum over the wave, the same on every lane.
 __device__ __forceinline__ double wave_sum_d(double v) {
-#pragma unroll
-    for (int o = 1; o < kWave; o <<= 1) v += shfl_xor_d(v, o);
-    return v;
+    v += dpp_d<kDppXor1>(v);
+    v += dpp_d<kDppXor2>(v);
+    v += dpp_d<kDppHalfMirror>(v);
+    v += dpp_d<kDppMirror>(v);
+    return (lane_d(v, 0) + lane_d(v, 16)) + (lane_d(v, 32) + lane_d(v, 48));
+}
+
+// exp(x) = 2^k e^r, k = round(x / ln 2), |r| <= ln(2) / 2, ln 2 in two parts
+// (the first its top 30 bits: k * it is exact), e^r by its Taylor polynomial of
+// degree 13 (what is left out is below 5e-18).  Clamped to where the result
+// is 0 or infinite.
+__device__ __forceinline__ double exp64(double x) {
+    x = fmin(fmax(x, -1000.0), 1000.0);
+    const double k = __builtin_rint(x * 1.4426950408889634);
+    double r = __builtin_fma(k, -0x1.62e42fe800000p-1, x);
+    r = __builtin_fma(k, -0x1.e8e7bcd5e4f1ep-31, r);
+    double p = 1.0 / 6227020800.0;
+    p = __builtin_fma(p, r, 1.0 / 479001600.0);
+    p = __builtin_fma(p, r, 1.0 / 39916800.0);
+    p = __builtin_fma(p, r, 1.0 / 3628800.0);
+    p = __builtin_fma(p, r, 1.0 / 362880.0);
+    p = __builtin_fma(p, r, 1.0 / 40320.0);
+    p = __builtin_fma(p, r, 1.0 / 5040.0);
+    p = __builtin_fma(p, r, 1.0 / 720.0);
+    p = __builtin_fma(p, r, 1.0 / 120.0);
+    p = __builtin_fma(p, r, 1.0 / 24.0);
+    p = __builtin_fma(p, r, 1.0 / 6.0);
+    p = __builtin_fma(p, r, 0.5);
+    p = __builtin_fma(p, r, 1.0);
+    p = __builtin_fma(p, r, 1.0);
+    return __builtin_amdgcn_ldexp(p, int(k));
 }
 
 // The order of doubles as that of their bits: key(a) < key(b) iff a < b.
@@ -45,32 +90,45 @@ __device__ __forceinline__ uint64_t order_key(double v) {
 
 constexpr double kOut = -__builtin_huge_val();   // an expert that cannot be picked
 
+__device__ __forceinline__ void wave_sync_lds() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// lpg: lanes of a group (64 without groups); V: experts of a lane.
 template <int NV, bool BF16>
 __global__ __launch_bounds__(kScWaves * kWave) void scores_kernel(ScoresArgs a, int lpg, int V) {
-    const int lane = threadIdx.x & (kWave - 1);
-    const int64_t t = int64_t(blockIdx.x) * kScWaves + threadIdx.x / kWave;
+    __shared__ double c_v[kScWaves][kWave];      // the gathered candidates
+    __shared__ int c_e[kScWaves][kWave];
+    __shared__ float c_l[kScWaves][kWave];
+    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+    const int64_t t = int64_t(blockIdx.x) * kScWaves + wave;
     if (t >= a.T) return;
     const int E = a.E, gsz = E / a.n_group;
+    const bool groups = a.n_group > 1;
     const int gi = lane / lpg, sub = lane - gi * lpg;
-    const int e0 = gi * gsz + sub * V;
-    int nv = gi < a.n_group ? min(V, gsz - sub * V) : 0;   // experts of this lane (may be <= 0)
+    // expert j of this lane is e0 + j * es, j < nv (nv may be <= 0)
+    const int e0 = groups ? gi * gsz + sub * V : lane, es = groups ? 1 : kWave;
+    const int nv = !groups ? (E - lane + kWave - 1) / kWave : gi < a.n_group ? min(V, gsz - sub * V) : 0;
 
-    auto logit = [&](int e) {
-        if constexpr (BF16) {
-            return bf16_to_f32(static_cast<const uint16_t*>(a.logits)[t * a.row_stride + e]);
-        } else {
-            const int64_t o = t * a.row_stride + e;
-            float l = static_cast<const float*>(a.logits)[o];
-            if (a.part1) l = (l + a.part1[o]) + (a.lbias ? a.lbias[e] : 0.0f);
-            return l;
-        }
-    };
     // an expert that is out: -inf; +inf is the largest finite logit
     auto clean = [](float l) { return l == l ? fminf(l, 3.402823466e+38f) : -__builtin_inff(); };
-
-    float lv[NV];
+    float lv[NV], bv[NV];
 #pragma unroll
-    for (int j = 0; j < NV; ++j) lv[j] = j < nv ? clean(logit(e0 + j)) : -__builtin_inff();
+    for (int j = 0; j < NV; ++j) {
+        const int e = j < nv ? e0 + j * es : 0;
+        const int64_t o = t * a.row_stride + e;
+        float l;
+        if constexpr (BF16) {
+            l = bf16_to_f32(static_cast<const uint16_t*>(a.logits)[o]);
+        } else {
+            l = static_cast<const float*>(a.logits)[o];
+            if (a.part1) l = (l + a.part1[o]) + (a.lbias ? a.lbias[e] : 0.0f);
+        }
+        bv[j] = a.bias ? a.bias[e] : 0.0f;
+        lv[j] = j < nv ? clean(l) : -__builtin_inff();
+    }
 
     double m = 0.0, iz = 1.0;   // softmax: the largest logit, 1 / sum exp(l - m)
     double v[NV];
@@ -78,14 +136,13 @@ __global__ __launch_bounds__(kScWaves * kWave) void scores_kernel(ScoresArgs a, 
         float lm = lv[0];
 #pragma unroll
         for (int j = 1; j < NV; ++j) lm = fmaxf(lm, lv[j]);
-        m = double(bits_f(0));
         const uint32_t k = wave_max_u32(score_key(lm));
         lm = (k & 0x80000000u) ? bits_f(k & 0x7FFFFFFFu) : bits_f(~k);
         m = lm > -__builtin_inff() ? double(lm) : 0.0;
         double z = 0.0;
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-            v[j] = j < V ? exp(double(lv[j]) - m) : 0.0;
+            v[j] = exp64(double(lv[j]) - m);      // -inf: 0
             z += v[j];
         }
         z = wave_sum_d(z);
@@ -94,15 +151,15 @@ __global__ __launch_bounds__(kScWaves * kWave) void scores_kernel(ScoresArgs a, 
         for (int j = 0; j < NV; ++j) v[j] *= iz;
     } else {
 #pragma unroll
-        for (int j = 0; j < NV; ++j) v[j] = j < V ? 1.0 / (1.0 + exp(-double(lv[j]))) : 0.0;
+        for (int j = 0; j < NV; ++j) v[j] = 1.0 / (1.0 + exp64(-double(lv[j])));
     }
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-        if (a.bias && j < nv) v[j] += double(a.bias[e0 + j]);
+        if (a.bias) v[j] += double(bv[j]);
         if (!(lv[j] > -__builtin_inff()) || v[j] != v[j]) v[j] = kOut;
     }
 
-    if (a.n_group > 1) {
+    if (groups) {
         double b1 = kOut, b2 = kOut;   // the two best of the lane, then of its group
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
@@ -117,8 +174,7 @@ __global__ __launch_bounds__(kScWaves * kWave) void scores_kernel(ScoresArgs a, 
         const double gs = a.top2 && b2 > kOut ? b1 + b2 : b1;
         int rank = 0;
         for (int g = 0; g < a.n_group; ++g) {
-            const double o = __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(gs), g * lpg),
-                                              __builtin_amdgcn_readlane(__double2loint(gs), g * lpg));
+            const double o = lane_d(gs, g * lpg);
             rank += (o > gs || (o == gs && g < gi)) ? 1 : 0;
         }
         if (rank >= a.topk_group) {
@@ -127,51 +183,102 @@ __global__ __launch_bounds__(kScWaves * kWave) void scores_kernel(ScoresArgs a, 
         }
     }
 
-    int my = -1;
+    // a bound that at least K experts reach, or all that are left
+    uint32_t key[NV], top = 0, bound = 1;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        key[j] = v[j] > kOut ? score_key(float(v[j])) : 0;
+        top = max(top, key[j]);
+    }
     for (int s = 0; s < a.K; ++s) {
-        double best = v[0];
-#pragma unroll
-        for (int j = 1; j < NV; ++j) best = fmax(best, v[j]);
-        const uint64_t key = order_key(best);
-        const uint32_t hi = uint32_t(key >> 32), lo = uint32_t(key);
-        const uint32_t whi = wave_max_u32(hi);
-        bool mine = hi == whi;
-        uint64_t bal = __ballot(mine);
-        if (bal & (bal - 1)) {                 // equal to 20 bits of mantissa: the low words decide
-            const uint32_t wlo = wave_max_u32(mine ? lo : 0u);
-            mine = mine && lo == wlo;
-            bal = __ballot(mine);
+        const uint32_t win = wave_max_u32(top);
+        if (win == 0) {                 // fewer than K lanes hold any
+            bound = 1;
+            break;
         }
-        const int owner = int(__builtin_ctzll(bal));
-        int slot = NV;
+        bound = win;
+        const int owner = int(__builtin_ctzll(__ballot(top == win)));
+        top = lane == owner ? 0 : top;
+    }
+    int n = 0;                          // candidates
 #pragma unroll
-        for (int j = NV - 1; j >= 0; --j)
-            if (v[j] == best) slot = j;
-        const int jw = __builtin_amdgcn_readlane(slot, owner);
-        const int ew = __builtin_amdgcn_readlane(e0, owner) + jw;
-        const bool none = __builtin_amdgcn_readlane(int(best == kOut), owner);
-        if (none) break;                       // nothing is left
-        if (lane == owner) {
-#pragma unroll
-            for (int j = 0; j < NV; ++j)
-                if (j == jw) v[j] = kOut;
+    for (int j = 0; j < NV; ++j) {
+        const uint64_t bal = __ballot(key[j] >= bound);
+        if (bal) {
+            const int pos = n + __builtin_amdgcn_mbcnt_hi(uint32_t(bal >> 32), __builtin_amdgcn_mbcnt_lo(uint32_t(bal), 0));
+            if (key[j] >= bound && pos < kWave) {
+                c_v[wave][pos] = v[j];
+                c_e[wave][pos] = e0 + j * es;
+                c_l[wave][pos] = lv[j];
+            }
+            n += __popcll(bal);
         }
-        if (lane == s) my = ew;
     }
 
-    // the picks' scores again, one a lane
-    double w = 0.0;
-    if (my >= 0) {
-        const double l = double(clean(logit(my)));
-        w = a.sigmoid ? 1.0 / (1.0 + exp(-l)) : exp(l - m) * iz;
+    int my = -1, slot = lane;           // this lane's pick and its place in the row
+    float ml = 0.0f;                    // its logit
+    if (n <= kWave) {
+        wave_sync_lds();
+        const bool live = lane < n;
+        const double cv = live ? c_v[wave][lane] : kOut;
+        const int ce = live ? c_e[wave][lane] : 0x7FFFFFFF;
+        int rank = 0;
+        for (int i = 0; i < n; ++i) {
+            const double ov = lane_d(cv, i);
+            const int oe = __builtin_amdgcn_readlane(ce, i);
+            rank += (ov > cv || (ov == cv && oe < ce)) ? 1 : 0;
+        }
+        slot = live ? rank : lane;      // lanes past the candidates: slots nothing is left for
+        if (live && rank < a.K) {
+            my = ce;
+            ml = c_l[wave][lane];
+        }
+    } else {
+        for (int s = 0; s < a.K; ++s) {
+            double best = v[0];
+#pragma unroll
+            for (int j = 1; j < NV; ++j) best = fmax(best, v[j]);
+            int jl = 0;                 // its first slot: the lane's lowest expert of that value
+#pragma unroll
+            for (int j = NV - 1; j >= 0; --j)
+                if (v[j] == best) jl = j;
+            const int e = e0 + jl * es;
+            const uint64_t k = order_key(best);
+            const uint32_t hi = uint32_t(k >> 32), lo = uint32_t(k);
+            // each maximum over all lanes, outside of any condition
+            const uint32_t whi = wave_max_u32(best > kOut ? hi : 0u);
+            if (whi == 0) break;                      // nothing is left
+            bool mine = best > kOut && hi == whi;
+            const uint32_t wlo = wave_max_u32(mine ? lo : 0u);
+            mine = mine && lo == wlo;
+            const uint32_t wne = wave_max_u32(mine ? ~uint32_t(e) : 0u);
+            mine = mine && ~uint32_t(e) == wne;
+            const int owner = int(__builtin_ctzll(__ballot(mine)));
+            const int we = __builtin_amdgcn_readlane(e, owner);
+            float wl = 0.0f;
+#pragma unroll
+            for (int j = 0; j < NV; ++j)
+                if (mine && j == jl) {
+                    v[j] = kOut;
+                    wl = lv[j];
+                }
+            wl = lane_f(wl, owner);
+            if (lane == s) {
+                my = we;
+                ml = wl;
+            }
+        }
     }
+
+    double w = 0.0;
+    if (my >= 0) w = a.sigmoid ? 1.0 / (1.0 + exp64(-double(ml))) : exp64(double(ml) - m) * iz;
     if (a.normalize) {
         const double z = wave_sum_d(w);
         w = z > 0.0 ? w / z : 0.0;
     }
-    if (lane < a.K) {
-        a.out_e[t * a.K + lane] = my;
-        a.out_w[t * a.K + lane] = float(w * double(a.scaling));
+    if (slot < a.K) {
+        a.out_e[t * a.K + slot] = my;
+        a.out_w[t * a.K + slot] = float(w * double(a.scaling));
     }
 }
 

@@ -298,23 +298,29 @@ def grouped_gemm_i8(w: Weight, N, swiglu, A, a_scale, out, offsets, counts, num_
 
 # ------------------------------------------------- router scores, block norms
 
+_f32, _b16, _i16 = torch.float32, torch.bfloat16, torch.int16
+_F32, _I32 = (_f32,), (torch.int32,)
+_B16 = (_b16, _i16)
+_FB16 = _F32 + _B16
+# the current device and its current stream's handle, without the wrapper
+# objects (1 us a call, as much as the rest of the checks)
+_device_now = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+_stream_now = (getattr(torch._C, "_cuda_getCurrentRawStream", None) or
+               (lambda dev: torch.cuda.current_stream(dev).cuda_stream))
+
+
 def _rows(t: torch.Tensor, what: str, width: int, rows: int):
     """(pointer, is bf16, row stride) of a [rows][width] tensor whose rows may
     lie apart; bf16 also as int16 bits, as elsewhere in this module."""
-    if t.dim() != 2 or t.shape[0] != rows or t.shape[1] != width:
+    if t.shape != (rows, width):
         raise _abi.GrimoireError(f"{what}: shape {tuple(t.shape)}, expected ({rows}, {width})")
-    st = t.stride()
-    if st[1] != 1 and width > 1:
+    apart, step = t.stride()
+    if step != 1 and width > 1:
         raise _abi.GrimoireError(f"{what}: elements of a row must be adjacent")
-    return t.data_ptr(), _bf16(t, what), (st[0] if rows > 1 else max(st[0], width))
-
-
-def _bf16(t: torch.Tensor, what: str) -> int:
-    if t.dtype is torch.float32:
-        return 0
-    if t.dtype is torch.bfloat16 or t.dtype is torch.int16:
-        return 1
-    raise _abi.GrimoireError(f"{what}: {t.dtype}, expected float32 or bfloat16")
+    d = t.dtype
+    if d is not _f32 and d is not _b16 and d is not _i16:
+        raise _abi.GrimoireError(f"{what}: {d}, expected float32 or bfloat16")
+    return t.data_ptr(), d is not _f32, apart if rows > 1 or apart > width else width
 
 
 def _flat(t: Optional[torch.Tensor], what: str, shape, dtypes, dev: int):
@@ -328,37 +334,17 @@ def _flat(t: Optional[torch.Tensor], what: str, shape, dtypes, dev: int):
     return t.data_ptr()
 
 
-_F32, _I32 = (torch.float32,), (torch.int32,)
-_B16 = (torch.bfloat16, torch.int16)
-_FB16 = _F32 + _B16
-
-
-class _On:
-    """Device `dev` as the current one for a launch on a stream of it."""
-    __slots__ = ("dev", "was")
-
-    def __init__(self, dev: int):
-        self.dev = dev
-
-    def __enter__(self):
-        self.was = torch.cuda.current_device()
-        if self.was != self.dev:
-            torch.cuda.set_device(self.dev)
-
-    def __exit__(self, *a):
-        if self.was != self.dev:
-            torch.cuda.set_device(self.was)
-
-
-def _launch(t: torch.Tensor, stream, fn, what: str, *args):
-    """Call entry point fn(stream, *args) on t's device and check its status."""
-    dev = t.get_device()
-    s = (stream if stream is not None else torch.cuda.current_stream(dev)).cuda_stream
-    if torch.cuda.current_device() == dev:
-        check(fn(s, *args), what)
+def _launch(dev: int, stream, fn, what: str, *args):
+    """Call entry point fn(stream, *args) with device dev current and check
+    its status; stream None: dev's current stream."""
+    s = _stream_now(dev) if stream is None else stream.cuda_stream
+    if _device_now() == dev:
+        r = fn(s, *args)
     else:
-        with _On(dev):
-            check(fn(s, *args), what)
+        with torch.cuda.device(dev):
+            r = fn(s, *args)
+    if r:
+        check(r, what)
 
 
 class RouteScores:
@@ -395,7 +381,7 @@ class RouteScores:
         lp, b16, stride = _rows(logits, "logits", E, T)
         if self.bias is not None and (self.bias.numel() != E or self.bias.get_device() != dev):
             raise _abi.GrimoireError("bias: one value an expert, on the logits' device")
-        _launch(logits, stream, lib().grimoire_moe_router_scores, "router_scores", self.struct, lp, b16, stride, T, E,
+        _launch(dev, stream, lib().grimoire_moe_router_scores, "router_scores", self.struct, lp, b16, stride, T, E,
                 K, _flat(out_expert, "out_expert", (T, K), _I32, dev),
                 _flat(out_weight, "out_weight", (T, K), _F32, dev))
 
@@ -445,7 +431,7 @@ class BlockNorm:
         xp, x16, stride = _rows(x, "x", H, T)
         if x.get_device() != dev:
             raise _abi.GrimoireError("x: on another device than h")
-        _launch(h, stream, lib().grimoire_block_norm, "block_norm", self.struct, gp, g16, hp, xp, x16, stride, hop, op,
+        _launch(dev, stream, lib().grimoire_block_norm, "block_norm", self.struct, gp, g16, hp, xp, x16, stride, hop, op,
                 obp, T, H)
 
     def moe(self, h, routed, inverse, route_weight, shared, h_out, out=None, out_bf=None, gate=None, stream=None):
@@ -455,7 +441,7 @@ class BlockNorm:
         if route_weight.dim() != 2:
             raise _abi.GrimoireError("route_weight: [T][K]")
         K = route_weight.shape[1]
-        _launch(h, stream, lib().grimoire_moe_block_norm, "moe_block_norm", self.struct, gp, g16, hp,
+        _launch(dev, stream, lib().grimoire_moe_block_norm, "moe_block_norm", self.struct, gp, g16, hp,
                 _flat(routed, "routed", (routed.shape[0], H), _B16, dev), routed.shape[0],
                 _flat(inverse.view(-1), "inverse", (T * K,), _I32, dev),
                 _flat(route_weight, "route_weight", (T, K), _F32, dev), _flat(shared, "shared", (T, H), _F32, dev), hop,
@@ -489,7 +475,7 @@ class Lora:
         xp, x16, xs = _rows(x, "x", A.K, T)
         bp, b16, bs = _rows(base, "base", A.N, T)
         yp, y16, ys = _rows(y, "output", width, T)
-        _launch(x, stream, fn, what, self.struct, _flat(row_slot, "row_slot", (T,), _I32, dev), xp, x16, xs, bp, b16,
+        _launch(dev, stream, fn, what, self.struct, _flat(row_slot, "row_slot", (T,), _I32, dev), xp, x16, xs, bp, b16,
                 bs, yp, y16, ys, T, self.workspace.data_ptr(), self.workspace.numel())
 
     def add(self, row_slot, x, y, base=None, stream=None):
