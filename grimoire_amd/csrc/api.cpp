@@ -545,6 +545,12 @@ static int lora_common(void* stream, const grim_lora* L, const int32_t* row_slot
     if (L->slots <= 0) return fail(GRIM_ERR_SHAPE, "slots=%d", L->slots);
     if (L->max_rank <= 0 || L->max_rank % 16 || L->max_rank > kLoraMaxRank)
         return fail(GRIM_ERR_SHAPE, "max_rank=%d (a multiple of 16, <= %d)", L->max_rank, kLoraMaxRank);
+    // the kernels address a slot and a tile of rows by 32 bits of bytes
+    if (int64_t(L->K > L->N ? L->K : L->N) * L->max_rank > int64_t(1) << 29)
+        return fail(GRIM_ERR_SHAPE, "K=%d N=%d max_rank=%d: a slot of more than 2^29 elements", L->K, L->N,
+                    L->max_rank);
+    if (x_stride > kLoraMaxStride || base_stride > kLoraMaxStride || y_stride > kLoraMaxStride)
+        return fail(GRIM_ERR_SHAPE, "row stride above %lld elements", (long long)kLoraMaxStride);
     const int width = glu ? L->N / 2 : L->N;
     if (x_stride < L->K || x_stride % 8) return fail(GRIM_ERR_SHAPE, "x_stride=%lld", (long long)x_stride);
     if (base_stride < L->N || base_stride % 4) return fail(GRIM_ERR_SHAPE, "base_stride=%lld", (long long)base_stride);

@@ -6,11 +6,17 @@
 // (and, for a gate|up projection, SwiGLU'd) on the way to y.
 //
 // Both are memory bound at every size (2 r operations an element of x and y
-// read or written), so the matrix cores are fed straight from memory: a tile
-// is 16 rows, and the lane pieces of A, B and x are MFMA operands as they
-// lie.  Rows of a tile that name different adapters are done one distinct
-// adapter after the other (long batches: runs of one request), or by one
-// work-group each (short batches, where rows are mixed).
+// read or written), and their rows go through the LDS on the way to the
+// matrix cores, so that adjacent lanes ask memory for adjacent pieces.  Rows
+// of a tile that name different adapters are done one distinct adapter after
+// the other, or by work-groups of their own.
+//
+// Where it stands (us, shrink + expand, and what their bytes take at the 4.94
+// TB/s of a large copy): 4096 rows of 9 requests, 2048 -> 7168, rank 64 of
+// mixed ranks, bf16: 13 + 35 (28; base copied to y by the same loop 25.5);
+// 2001 rows of 5, 2880 -> 2 x 2880, rank 16, fp32: 11 + 19 (19); 48 mixed
+// rows of 32 adapters, 2048 -> 7168: 6 + 12 (3.3); one row: 4 + 5, two
+// dependent chains of loads.
 //
 // fp32 values are multiplied exactly: an fp32 x (and z) is the sum of three
 // bf16 pieces of 8 significant bits, cut off, not rounded, so each rest is
@@ -23,17 +29,14 @@ namespace {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-// 16 bytes from an 8-byte aligned row (one load: global accesses need 4)
-typedef uint32_t u32x4_a8 __attribute__((ext_vector_type(4), aligned(8)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 
 constexpr int kRows = 16;        // rows of a tile
 constexpr int kStep = 64;        // shrink: k of one step of a wave, 16 a lane
 constexpr int kShrinkWaves = 8;
 constexpr int kExpandWaves = 4;
-constexpr int kCols = 32;        // expand: columns of one block of a wave
-// Batches of up to this many rows give every distinct adapter of a tile its
-// own work-groups.
+// shrink: batches of up to this many rows give every distinct adapter of a
+// tile a work-group of its own.
 constexpr int kItemRows = 512;
 constexpr int kMaxSplits = 8;
 
@@ -66,19 +69,20 @@ __device__ __forceinline__ void pieces(float (&v)[8], u32x4 (&o)[3]) {
     }
 }
 
-// The rows of a tile and the adapters they name: lane l (and l+16, l+32,
-// l+48) holds row l's.
+// The rows of a tile of ROWS (16 or 64) and the adapters they name: lane l
+// holds row l % ROWS's.
 struct Tile {
     int row;      // this lane's row, clamped into the batch
     bool in;      // the row exists
     int slot;     // its adapter or -1
 };
 
+template <int ROWS>
 __device__ __forceinline__ Tile tile_rows(const LoraArgs& p, int tile) {
-    const int r = tile * kRows + (threadIdx.x & 15);
+    const int64_t r = int64_t(tile) * ROWS + (threadIdx.x & (ROWS - 1));
     Tile t;
     t.in = r < p.T;
-    t.row = t.in ? r : p.T - 1;
+    t.row = t.in ? int(r) : p.T - 1;
     const int s = p.row_slot[t.row];
     t.slot = t.in && s >= 0 && s < p.slots ? s : -1;
     return t;
@@ -93,63 +97,101 @@ __device__ __forceinline__ int next_slot(const Tile& t, uint64_t& todo, int& lea
     return s;
 }
 
+__device__ __forceinline__ void wave_sync_lds() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// The workspace holds z as expand's operands: per split, tile of 16 rows and
+// 32 ranks two runs of 64 lanes' four values; expand's lane (q, col) takes
+// ranks 8 q .. 8 q + 3 of row col from the first, the next four from the
+// second.  This is where shrink's lane (q, col), with ranks 4 q .. 4 q + 3 of
+// fragment f, puts its own.
+__device__ __forceinline__ f32x4* z_run(const LoraArgs& p, int split, int64_t tile, int chunk, int half) {
+    const int chunks = (p.R + 31) / 32;
+    const int64_t tiles = (p.T + kRows - 1) / kRows;
+    return reinterpret_cast<f32x4*>(p.part) + (((split * tiles + tile) * chunks + chunk) * 2 + half) * kWave;
+}
+__device__ __forceinline__ f32x4* z_at(const LoraArgs& p, int split, int64_t tile, int f, int q, int col) {
+    return z_run(p, split, tile, f >> 1, q & 1) + ((f & 1) * 2 + (q >> 1)) * 16 + col;
+}
+
 // ------------------------------------------------------------------ shrink
 
 // A wave's share of z = A x: NF fragments of 16 ranks, the K steps s0, s0 +
-// kShrinkWaves, ... < s1, two at a time so that both are in flight.  All
-// loads are unconditional: a step past the end and k past K read memory the
-// wave reads anyway, under an x of zero; ranks past the slot read its last
-// row, and are not stored.
+// kShrinkWaves, ... < s1, the next one's loads in flight while one is used.
+// As in expand, A and x go through the LDS so that adjacent lanes load
+// adjacent pieces of a row (as operands every lane would load from a row of
+// its own: 64 tag look-ups an instruction; 16.4 against 10.9 us at 4096
+// rows of one adapter, K 2048, rank 64).  A row's pieces are permuted by its
+// number, so that the 16 rows of an operand lie in different banks.  All
+// loads are unconditional: k past K reads the row's end under an x of zero, ranks past
+// the slot read its last row and are not stored.
 template <bool XB, int NF>
-__device__ __forceinline__ void shrink_steps(const void* xrow, const uint16_t* aslot, int64_t K, int rows, int col,
-                                             int q, int s0, int s1, f32x4 (&acc)[4]) {
-    constexpr int XV = XB ? 2 : 4;
-    const uint16_t* ap[NF];
+__device__ __forceinline__ void shrink_steps(const LoraArgs& p, int slot, int r0, uint32_t mask, int64_t row0,
+                                             int lead, int lane, int s0, int s1, u32x4* lds, f32x4 (&acc)[4]) {
+    constexpr int XP = XB ? 8 : 16, XL = XP / 4;          // pieces of an x row, its loads
+    const int q = lane >> 4, col = lane & 15;
+    u32x4* xl = lds + NF * 16 * 8;
+    const char* as = reinterpret_cast<const char*>(p.a + (int64_t(slot) * p.R + r0) * p.K);
+    const char* xs = static_cast<const char*>(p.x) + row0 * p.x_stride * (XB ? 2 : 4);
+    uint32_t ao[NF * 2], xo[XL];
 #pragma unroll
-    for (int r = 0; r < NF; ++r) ap[r] = aslot + min(r * 16 + col, rows - 1) * K;
-    for (int s = s0; s < s1; s += 2 * kShrinkWaves) {
-        u32x4 x[2][XV], a[2][NF][2];
+    for (int i = 0; i < NF * 2; ++i) ao[i] = uint32_t(min(i * 8 + (lane >> 3), p.R - r0 - 1)) * p.K * 2u;
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const int k = min(s + u * kShrinkWaves, s1 - 1) * kStep + q * 8;
+    for (int i = 0; i < XL; ++i) {
+        // rows of another adapter read the group's first row instead: their
+        // column of the product is not used
+        const int r = i * (kWave / XP) + lane / XP;
+        xo[i] = uint32_t((mask >> r) & 1 ? r : lead) * uint32_t(p.x_stride) * (XB ? 2u : 4u);
+    }
+    u32x4 a[NF * 2], x[XL];
+    auto load = [&](int s) {
+        const uint32_t ak = min(s * kStep + (lane & 7) * 8, p.K - 8) * 2u;
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int64_t kk = min(int64_t(k + h * 32), K - 8);
-                if constexpr (XB) {
-                    x[u][h] = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(xrow) + kk);
-                } else {
-                    const float* xp = static_cast<const float*>(xrow) + kk;
-                    x[u][h * 2] = *reinterpret_cast<const u32x4*>(xp);
-                    x[u][h * 2 + 1] = *reinterpret_cast<const u32x4*>(xp + 4);
-                }
+        for (int i = 0; i < NF * 2; ++i) a[i] = *reinterpret_cast<const u32x4*>(as + (ao[i] + ak));
+        const uint32_t xk = XB ? ak : min(s * kStep + (lane & 15) * 4, p.K - 4) * 4u;
 #pragma unroll
-                for (int r = 0; r < NF; ++r) a[u][r][h] = *reinterpret_cast<const u32x4*>(ap[r] + kk);
-            }
+        for (int i = 0; i < XL; ++i) x[i] = *reinterpret_cast<const u32x4*>(xs + (xo[i] + xk));
+    };
+    if (s0 < s1) load(s0);
+#pragma nounroll
+    for (int s = s0; s < s1; s += kShrinkWaves) {
+        const bool in = s * kStep + (lane % XP) * (XB ? 8 : 4) < p.K;
+#pragma unroll
+        for (int i = 0; i < NF * 2; ++i) lds[(i * 8 + (lane >> 3)) * 8 + ((lane & 7) ^ (lane >> 3))] = a[i];
+#pragma unroll
+        for (int i = 0; i < XL; ++i) {
+            const int r = i * (kWave / XP) + lane / XP;
+            xl[r * XP + ((lane % XP) ^ (r & (XP - 1)))] = in ? x[i] : u32x4{0, 0, 0, 0};
         }
+        wave_sync_lds();
+        load(min(s + kShrinkWaves, s1 - 1));               // past the end: memory read already
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const int k = (s + u * kShrinkWaves) * kStep + q * 8;
+        for (int h = 0; h < 2; ++h) {
+            u32x4 xv[3];
+            if constexpr (XB) {
+                xv[0] = xl[col * 8 + ((h * 4 + q) ^ (col & 7))];
+            } else {
+                const u32x4 lo = xl[col * 16 + ((h * 8 + q * 2) ^ col)], hi = xl[col * 16 + ((h * 8 + q * 2 + 1) ^ col)];
+                float v[8];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const bool in = s + u * kShrinkWaves < s1 && k + h * 32 < K;
-                u32x4 xv[3];
-                if constexpr (XB) {
-                    xv[0] = in ? x[u][h] : u32x4{0, 0, 0, 0};
-                } else {
-                    float v[8];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        v[i] = in ? bits_f(x[u][h * 2][i]) : 0.0f;
-                        v[4 + i] = in ? bits_f(x[u][h * 2 + 1][i]) : 0.0f;
-                    }
-                    pieces(v, xv);
+                for (int i = 0; i < 4; ++i) {
+                    v[i] = bits_f(lo[i]);
+                    v[4 + i] = bits_f(hi[i]);
                 }
-#pragma unroll
-                for (int l = XB ? 0 : 2; l >= 0; --l)
-#pragma unroll
-                    for (int r = 0; r < NF; ++r) acc[r] = mfma(a[u][r][h], xv[l], acc[r]);
+                pieces(v, xv);
             }
+            u32x4 av[NF];
+#pragma unroll
+            for (int r = 0; r < NF; ++r) av[r] = lds[(r * 16 + col) * 8 + ((h * 4 + q) ^ (col & 7))];
+#pragma unroll
+            for (int l = XB ? 0 : 2; l >= 0; --l)
+#pragma unroll
+                for (int r = 0; r < NF; ++r) acc[r] = mfma(av[r], xv[l], acc[r]);
         }
+        wave_sync_lds();
     }
 }
 
@@ -157,12 +199,13 @@ __device__ __forceinline__ void shrink_steps(const void* xrow, const uint16_t* a
 template <bool XB, int NR>
 __global__ __launch_bounds__(kShrinkWaves * kWave) void lora_shrink_kernel(LoraArgs p, int splits, int ksteps,
                                                                            int chunks, int items) {
-    __shared__ f32x4 red[kShrinkWaves][NR][kWave];
+    // a wave's A and x; at the end its fragments of z, for the sum over waves
+    __shared__ u32x4 lds[kShrinkWaves][NR * 16 * 8 + kRows * (XB ? 8 : 16)];
     const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
     const int q = lane >> 4, col = lane & 15;
     const int tile = blockIdx.x, split = blockIdx.y;
     const int chunk = blockIdx.z % chunks, item = blockIdx.z / chunks;
-    const Tile t = tile_rows(p, tile);
+    const Tile t = tile_rows<kRows>(p, tile);
     uint64_t todo = __ballot(t.slot >= 0) & 0xFFFFu;
     // the split's steps [s0, s1), dealt to the waves in turn
     const int per = (ksteps + splits - 1) / splits;
@@ -177,28 +220,30 @@ __global__ __launch_bounds__(kShrinkWaves * kWave) void lora_shrink_kernel(LoraA
         const int nr = min(NR, (rank - r0 + 15) / 16);      // fragments with live ranks
         if (nr > 0) {
             f32x4 acc[4] = {};
-            // rows of another adapter read the group's first row instead:
-            // their column of the product is not used
-            const bool mine = t.slot == slot;
-            const int64_t xo = int64_t(mine ? t.row : __builtin_amdgcn_readlane(t.row, lead)) * p.x_stride;
-            const void* xrow = XB ? static_cast<const void*>(static_cast<const uint16_t*>(p.x) + xo)
-                                  : static_cast<const void*>(static_cast<const float*>(p.x) + xo);
-            const uint16_t* as = p.a + (int64_t(slot) * p.R + r0) * p.K;
-            if (NR == 1 || nr == 1) shrink_steps<XB, 1>(xrow, as, p.K, p.R - r0, col, q, s0, s1, acc);
-            else if (NR == 2 || nr == 2) shrink_steps<XB, 2>(xrow, as, p.K, p.R - r0, col, q, s0, s1, acc);
-            else shrink_steps<XB, 4>(xrow, as, p.K, p.R - r0, col, q, s0, s1, acc);
+            const uint32_t mask = uint32_t(__ballot(t.slot == slot)) & 0xFFFFu;
+            int ln = lane;                                  // opaque: see expand_cols
+            asm volatile("" : "+v"(ln));
+#define GRIM_STEPS(NF) \
+    shrink_steps<XB, NF>(p, slot, r0, mask, int64_t(tile) * kRows, lead, ln, s0, s1, lds[wave], acc)
+            if (NR == 1 || nr == 1) GRIM_STEPS(1);
+            else if (NR == 2 || nr == 2) GRIM_STEPS(2);
+            else GRIM_STEPS(4);
+#undef GRIM_STEPS
 #pragma unroll
             for (int r = 0; r < NR; ++r)
-                if (r < nr) red[wave][r][lane] = acc[r];
+                if (r < nr) __builtin_memcpy(&lds[wave][r * kWave + lane], &acc[r], 16);
             __syncthreads();
             // D of a fragment: lane (q, col) holds ranks 4q .. 4q+3 of row
             // col, and wave r sums fragment r over the waves
             if (wave < nr) {
-                f32x4 z = red[0][wave][lane];
+                f32x4 z = {};
 #pragma unroll
-                for (int w = 1; w < kShrinkWaves; ++w) z += red[w][wave][lane];
-                if (mine)
-                    *reinterpret_cast<f32x4*>(p.part + (int64_t(split) * p.T + t.row) * p.R + r0 + wave * 16 + q * 4) = z;
+                for (int w = 0; w < kShrinkWaves; ++w) {
+                    f32x4 o;
+                    __builtin_memcpy(&o, &lds[w][wave * kWave + lane], 16);
+                    z += o;
+                }
+                if (t.slot == slot) *z_at(p, split, tile, (r0 >> 4) + wave, q, col) = z;
             }
             __syncthreads();
         }
@@ -215,38 +260,6 @@ __device__ __forceinline__ float glu(float g, float u) {
     return g * __builtin_amdgcn_rcpf(1.0f + e) * u;
 }
 
-// Eight columns of a base row: n .. n+7, of which the first four or all
-// (whole) exist.
-template <bool BB>
-struct Base {
-    u32x4 v[BB ? 1 : 2];
-};
-
-template <bool BB>
-__device__ __forceinline__ void load_base(Base<BB>& b, const void* base, int64_t o, bool whole) {
-    if constexpr (BB) {
-        const uint16_t* p = static_cast<const uint16_t*>(base) + o;
-        if (whole) {
-            b.v[0] = *reinterpret_cast<const u32x4_a8*>(p);
-        } else {
-            const uint2 u = *reinterpret_cast<const uint2*>(p);
-            b.v[0] = u32x4{u.x, u.y, 0, 0};
-        }
-    } else {
-        const float* p = static_cast<const float*>(base) + o;
-        b.v[0] = *reinterpret_cast<const u32x4*>(p);
-        b.v[1] = *reinterpret_cast<const u32x4*>(p + (whole ? 4 : 0));
-    }
-}
-
-template <bool BB>
-__device__ __forceinline__ float base_at(const Base<BB>& b, int i) {
-    if constexpr (BB)
-        return i & 1 ? bits_f(b.v[0][i / 2] & 0xFFFF0000u) : bits_f(b.v[0][i / 2] << 16);
-    else
-        return bits_f(b.v[i / 4][i & 3]);
-}
-
 // two fp32 to bf16, nearest even (the hardware conversion)
 __device__ __forceinline__ uint32_t bf16_pair(float lo, float hi) {
     const bf16x2 b = __builtin_convertvector(f32x2{lo, hi}, bf16x2);
@@ -255,170 +268,272 @@ __device__ __forceinline__ uint32_t bf16_pair(float lo, float hi) {
     return u;
 }
 
-__device__ __forceinline__ void store8(void* y, int64_t o, int bf16, const float (&v)[8], bool whole) {
+// W columns of a base row as loaded (2 or 4, fp32 or bf16).
+template <bool BB, int W>
+struct Base {
+    uint32_t v[BB ? W / 2 : W];
+};
+
+// Memory is addressed as a pointer all lanes share and 32 bits of byte
+// offset (the entry points bound strides and adapters so that it fits).
+template <bool BB, int W>
+__device__ __forceinline__ void load_base(Base<BB, W>& b, const void* base, uint32_t off) {
+    __builtin_memcpy(b.v, __builtin_assume_aligned(static_cast<const char*>(base) + off, BB ? 2 * W : 4 * W), sizeof b.v);
+}
+
+template <bool BB, int W>
+__device__ __forceinline__ float base_at(const Base<BB, W>& b, int i) {
+    if constexpr (BB) return i & 1 ? bits_f(b.v[i / 2] & 0xFFFF0000u) : bits_f(b.v[i / 2] << 16);
+    else return bits_f(b.v[i]);
+}
+
+// columns at element `off` past y
+template <int W>
+__device__ __forceinline__ void store_cols(void* y, uint32_t off, int bf16, const float (&v)[W]) {
     if (bf16) {
-        uint16_t* p = static_cast<uint16_t*>(y) + o;
-        u32x4 u;
+        uint32_t u[W / 2];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) u[i] = bf16_pair(v[2 * i], v[2 * i + 1]);
-        if (whole) *reinterpret_cast<u32x4_a8*>(p) = u;
-        else *reinterpret_cast<uint2*>(p) = make_uint2(u[0], u[1]);
+        for (int i = 0; i < W / 2; ++i) u[i] = bf16_pair(v[2 * i], v[2 * i + 1]);
+        __builtin_memcpy(__builtin_assume_aligned(static_cast<char*>(y) + off * 2u, 2 * W), u, sizeof u);
     } else {
-        float* p = static_cast<float*>(y) + o;
-        *reinterpret_cast<f32x4*>(p) = f32x4{v[0], v[1], v[2], v[3]};
-        if (whole) *reinterpret_cast<f32x4*>(p + 4) = f32x4{v[4], v[5], v[6], v[7]};
+        __builtin_memcpy(__builtin_assume_aligned(static_cast<char*>(y) + off * 4u, 4 * W), v, sizeof v);
     }
 }
 
-// One group of rows of a tile (one adapter, or none) against columns
+// A work-group takes 64 rows, 16 a wave.  A block is 64 rows of B: 64 columns
+// of y, or 32 and the 32 beside them of the up half.  Four MFMA tiles of 16;
+// tile j's column n is column 4 n + j of the block (gate|up: column 2 n +
+// j % 2 of half j / 2), so that a lane's results are adjacent columns and a
+// row's base and y are runs of memory over adjacent lanes.
+//
+// B goes through the LDS, once for the four waves: as operands (lane =
+// column, 16 bytes of its ranks) its loads would touch a row a lane, 64 tag
+// look-ups an instruction, which bound this kernel; adjacent lanes read
+// adjacent pieces instead.  A row of the LDS is 16 bytes longer than its
+// ranks, an odd number of pieces: the 16 rows of a tile's read lie in
+// different banks.
+constexpr int kExpandRows = kExpandWaves * kRows;
+constexpr int kThreads = kExpandWaves * kWave;
+template <bool GLU>
+__device__ __forceinline__ int block_col(int r) {      // block row -> its column of y (and half)
+    return GLU ? (r & 31) : r;
+}
+template <bool GLU>
+__device__ __forceinline__ int lds_row(int r) {        // -> its place: tile by tile
+    return GLU ? ((r >> 5) * 2 + (r & 1)) * 16 + ((r & 31) >> 1) : (r & 3) * 16 + (r >> 2);
+}
+
+// The wave's rows `mask` of one adapter (of none: slot -1) against columns
 // [first, last) of y: CC chunks of 32 ranks (HALF: max_rank 16, where an
 // instruction's 32 k hold the 16 ranks twice, under two pieces of z; CC 0:
-// base alone), G blocks of 32 columns at a time whose base is requested
-// together.  A block is two MFMA tiles of 16 columns, tile j's operand row m
-// being column 8 (m / 4) + 4 j + m % 4, so that a lane's part of the two
-// products is eight columns in a row.
-template <bool GLU, int CC, bool HALF, bool BB, int G>
-__device__ __forceinline__ void expand_cols(const LoraArgs& p, int splits, int slot, int rank, int row, int lead_row,
-                                            bool mine, int q, int col, int first, int last, int width) {
-    constexpr int NP = GLU ? 2 : 1, C = CC ? CC : 1;
-    // rows of other groups read the first row's z and base, and do not store
-    const int64_t src = mine ? row : lead_row;
-    // z, scaled and without what lies past the rank, in three pieces
+// base alone).  All waves of the work-group come here together, also those
+// without such rows (mask 0), which only bring B.
+template <bool GLU, int CC, bool HALF, bool BB>
+__device__ __forceinline__ void expand_cols(const LoraArgs& p, int splits, int slot, int rank, uint32_t mask,
+                                            int64_t row0, int first, int last, int width, u32x4* lds) {
+    constexpr int W = GLU ? 2 : 4, NP = GLU ? 2 : 1, C = CC ? CC : 1;
+    constexpr int PH = C < 2 ? C : 2;                 // chunks of one pass through the LDS
+    constexpr int P = HALF ? 2 : PH * 4;              // pieces of a row in a pass
+    constexpr int kPitch = P + 1, kBuffer = 64 * kPitch;
+    constexpr int L = (64 * P + kThreads - 1) / kThreads;   // loads a thread and pass
+    // (opaque: what hangs on the lane is formed here, not kept in registers
+    // for every rank's code from before the loop over the adapters)
+    int tid = threadIdx.x;
+    asm volatile("" : "+v"(tid));
+    const int lane = tid & (kWave - 1), q = lane >> 4, col = lane & 15;
+
+    // the four rows of this lane's results; rows that are not stored read
+    // the first stored one's base
+    constexpr uint32_t ES = BB ? 2 : 4;
+    const char* base0 = static_cast<const char*>(p.base) + row0 * p.base_stride * ES;
+    char* y0 = static_cast<char*>(p.y) + row0 * p.y_stride * (p.y_bf16 ? 2 : 4);
+    const uint32_t brow = uint32_t(p.base_stride) * ES, yrow = uint32_t(p.y_stride);
+    const int lead = mask ? __builtin_ctz(mask) : 0;
+    auto mine = [&](int i) { return (mask >> (q * 4 + i)) & 1; };
+    auto row = [&](int i) { return uint32_t(mine(i) ? q * 4 + i : lead); };
+
+    // a pass's B: thread reads piece % P of rows tid / P, + 256 / P
+    const uint16_t* bs = p.b + int64_t(slot) * p.N * p.R;
+    auto load_b = [&](u32x4 (&d)[L], int n0, int c0) {
+        const uint32_t pitch = p.R * 2u, r = min((HALF ? 0 : c0 * 32) + (tid % P) * 8, p.R - 8) * 2u;
+        const uint32_t end = (width - 1) * pitch + r;      // the last column's
+#pragma unroll
+        for (int i = 0; i < L; ++i) {
+            const int br = (i * (kThreads / P) + tid / P) & 63;
+            const uint32_t o = min((n0 + block_col<GLU>(br)) * pitch + r, end) + (GLU && br >= 32 ? width * pitch : 0u);
+            d[i] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(bs) + o);
+        }
+    };
+    auto load_y = [&](Base<BB, W> (&d)[NP][4], int n0) {
+        const uint32_t n = min(n0 + col * W, width - W) * ES;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int h = 0; h < NP; ++h) load_base<BB, W>(d[h][i], base0 + h * width * ES, row(i) * brow + n);
+    };
+
+    constexpr int kBlock = GLU ? 32 : 64;
+    u32x4 b[L];
+    Base<BB, W> base[NP][4] = {};
+    if (mask) load_y(base, first);
+    if constexpr (CC > 0) load_b(b, first, 0);
+
+    // z of row `col`, ranks q * 8 .. + 7 of each chunk, scaled and without
+    // what lies past the rank, in three pieces (rows of other adapters hold
+    // anything: their rows of the product are not stored)
     u32x4 zv[C][3];
     if constexpr (CC > 0) {
-        const float scale = p.scale[slot];
+        if (mask) {
+            const float scale = p.scale[slot];
 #pragma unroll
-        for (int c = 0; c < C; ++c) {
-            const int r = HALF ? (q & 1) * 8 : c * 32 + q * 8;
-            const float* zp = p.part + src * p.R + min(r, p.R - 8);
-            f32x4 lo = {}, hi = {};
-            for (int s = 0; s < splits; s += 4) {
-                f32x4 l[4], h[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float* sp = zp + int64_t(min(s + i, splits - 1)) * p.T * p.R;
-                    l[i] = *reinterpret_cast<const f32x4*>(sp);
-                    h[i] = *reinterpret_cast<const f32x4*>(sp + 4);
-                }
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (s + i < splits) {
-                        lo += l[i];
-                        hi += h[i];
+            for (int c = 0; c < C; ++c) {
+                const int r = HALF ? (q & 1) * 8 : c * 32 + q * 8;
+                const int64_t apart = z_run(p, 1, 0, 0, 0) - z_run(p, 0, 0, 0, 0);
+                const f32x4* z0 = z_run(p, 0, row0 / kRows, c, 0) + (HALF ? lane & 31 : lane);
+                f32x4 lo = {}, hi = {};
+                for (int s = 0; s < splits; s += 2) {
+                    const f32x4* z1 = z0 + s * apart;
+                    const f32x4* z2 = z0 + min(s + 1, splits - 1) * apart;
+                    const f32x4 l1 = z1[0], h1 = z1[kWave], l2 = z2[0], h2 = z2[kWave];
+                    lo += l1;
+                    hi += h1;
+                    if (s + 1 < splits) {
+                        lo += l2;
+                        hi += h2;
                     }
-            }
-            float z[8];
+                }
+                float z[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) z[i] = r + i < rank ? (i < 4 ? lo[i & 3] : hi[i & 3]) * scale : 0.0f;
-            pieces(z, zv[c]);
-            if constexpr (HALF) {
-                zv[c][0] = q < 2 ? zv[c][0] : zv[c][1];
-                zv[c][1] = q < 2 ? zv[c][2] : u32x4{0, 0, 0, 0};
+                for (int i = 0; i < 8; ++i) z[i] = r + i < rank ? (i < 4 ? lo[i & 3] : hi[i & 3]) * scale : 0.0f;
+                pieces(z, zv[c]);
+                if constexpr (HALF) {
+                    zv[c][0] = q < 2 ? zv[c][0] : zv[c][1];
+                    zv[c][1] = q < 2 ? zv[c][2] : u32x4{0, 0, 0, 0};
+                }
             }
         }
     }
-    const uint16_t* bs = p.b + int64_t(slot) * p.N * p.R;
-    const int64_t bo = src * p.base_stride, yo = int64_t(row) * p.y_stride;
-    const int ncol = 8 * (col >> 2) + (col & 3);
 
-    for (int n0 = first; n0 < last; n0 += G * kCols) {
-        Base<BB> base[G][NP];
+    int turn = 0;
+#pragma nounroll
+    for (int n0 = first; n0 < last; n0 += kBlock) {
+        const int next = n0 + kBlock < last ? n0 + kBlock : n0;   // past the end: memory read already
+        // -0: what adds nothing leaves base's own sign of zero
+        f32x4 acc[4];
 #pragma unroll
-        for (int g = 0; g < G; ++g) {
-            const int n = min(n0 + g * kCols + q * 8, width - 4);
+        for (int i = 0; i < 4; ++i) acc[i] = f32x4{-0.0f, -0.0f, -0.0f, -0.0f};
+        Base<BB, W> cur[NP][4];
 #pragma unroll
-            for (int h = 0; h < NP; ++h) load_base<BB>(base[g][h], p.base, bo + n + h * width, n + 8 <= width);
+        for (int h = 0; h < NP; ++h)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) cur[h][i] = base[h][i];
+        if constexpr (CC > 0) {
+#pragma unroll
+            for (int c0 = 0; c0 < C; c0 += PH, turn ^= 1) {
+                // what lies past the rank is not part of the adapter
+                const int r = (HALF ? 0 : c0 * 32) + (tid % P) * 8;
+                if (rank < c0 * 32 + P * 8) {
+#pragma unroll
+                    for (int i = 0; i < L; ++i)
+#pragma unroll
+                        for (int d = 0; d < 4; ++d) {
+                            uint32_t w = b[i][d];
+                            w = r + 2 * d + 1 < rank ? w : w & 0xFFFFu;
+                            b[i][d] = r + 2 * d < rank ? w : 0u;
+                        }
+                }
+                // two buffers in turn: who writes one has passed the barrier
+                // that every wave reached after its reads of it
+                u32x4* buf = lds + turn * kBuffer;
+#pragma unroll
+                for (int i = 0; i < L; ++i) {
+                    const int br = i * (kThreads / P) + tid / P;
+                    if (64 * P % kThreads == 0 || br < 64) buf[lds_row<GLU>(br) * kPitch + tid % P] = b[i];
+                }
+                __syncthreads();
+                const bool more = c0 + PH < C;
+                load_b(b, more ? n0 : next, more ? c0 + PH : 0);
+                if (!mask) continue;
+                if (c0 == 0) load_y(base, next);
+#pragma unroll
+                for (int c = 0; c < PH; ++c) {
+                    u32x4 d[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) d[j] = buf[(j * 16 + col) * kPitch + (HALF ? q & 1 : c * 4 + q)];
+#pragma unroll
+                    for (int l = HALF ? 1 : 2; l >= 0; --l)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) acc[j] = mfma(zv[c0 + c][l], d[j], acc[j]);
+                }
+            }
+        } else {
+            if (mask) load_y(base, next);
         }
-        u32x4 b[2][C][NP][2];
-        auto load_b = [&](u32x4 (&d)[C][NP][2], int nb) {
+        // D of tile j: lane (q, col) holds rows 4q .. 4q+3 of its column
+        const int n = n0 + col * W;
+        if (mask && n < width) {
 #pragma unroll
-            for (int c = 0; c < CC; ++c) {
-                const int r = HALF ? (q & 1) * 8 : min(c * 32 + q * 8, p.R - 8);
+            for (int i = 0; i < 4; ++i) {
+                float v[W];
 #pragma unroll
-                for (int h = 0; h < NP; ++h)
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        const int n = min(nb + ncol + 4 * j, width - 1) + h * width;
-                        d[c][h][j] = *reinterpret_cast<const u32x4*>(bs + int64_t(n) * p.R + r);
-                    }
-            }
-        };
-        load_b(b[0], n0);
-#pragma unroll
-        for (int g = 0; g < G; ++g) {
-            if (g + 1 < G) load_b(b[(g + 1) & 1], n0 + (g + 1) * kCols);
-            // -0: what adds nothing leaves base's own sign of zero
-            f32x4 acc[NP][2];
-#pragma unroll
-            for (int h = 0; h < NP; ++h)
-#pragma unroll
-                for (int j = 0; j < 2; ++j) acc[h][j] = f32x4{-0.0f, -0.0f, -0.0f, -0.0f};
-#pragma unroll
-            for (int c = 0; c < CC; ++c) {
-                u32x4(&d)[NP][2] = b[g & 1][c];
-                if (rank < c * 32 + (HALF ? 16 : 32)) {     // what lies past the rank, whatever it is
-                    const int r = HALF ? (q & 1) * 8 : c * 32 + q * 8;
-#pragma unroll
-                    for (int h = 0; h < NP; ++h)
-#pragma unroll
-                        for (int j = 0; j < 2; ++j)
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                uint32_t w = d[h][j][i];
-                                w = r + 2 * i + 1 < rank ? w : w & 0xFFFFu;
-                                d[h][j][i] = r + 2 * i < rank ? w : 0u;
-                            }
+                for (int w = 0; w < W; ++w) {
+                    v[w] = base_at<BB, W>(cur[0][i], w) + acc[w][i];
+                    if constexpr (GLU) v[w] = glu(v[w], base_at<BB, W>(cur[NP - 1][i], w) + acc[2 + w][i]);
                 }
-#pragma unroll
-                for (int l = HALF ? 1 : 2; l >= 0; --l)
-#pragma unroll
-                    for (int h = 0; h < NP; ++h)
-#pragma unroll
-                        for (int j = 0; j < 2; ++j) acc[h][j] = mfma(d[h][j], zv[c][l], acc[h][j]);
-            }
-            // D: lane (q, col) holds columns 8q + 4j .. + 3 of row col
-            const int n = n0 + g * kCols + q * 8;
-            if (mine && n < width) {
-                float v[8];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    v[i] = base_at<BB>(base[g][0], i) + acc[0][i / 4][i & 3];
-                    if constexpr (GLU) v[i] = glu(v[i], base_at<BB>(base[g][NP - 1], i) + acc[NP - 1][i / 4][i & 3]);
-                }
-                store8(p.y, yo + n, p.y_bf16, v, n + 8 <= width);
+                if (mine(i)) store_cols<W>(y0, row(i) * yrow + n, p.y_bf16, v);
             }
         }
     }
+    if constexpr (CC > 0) __syncthreads();             // the next adapter starts at the first buffer
 }
 
 // MC: chunks of 32 ranks of max_rank (0: max_rank 16); a group of rows takes
 // the code of its own adapter's rank.
-template <bool GLU, int MC, bool BB, int G>
-__global__ __launch_bounds__(kExpandWaves * kWave) void lora_expand_kernel(LoraArgs p, int splits, int items,
-                                                                           int wave_rows, int cgroups, int ngroups) {
-    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
-    const int q = lane >> 4, col = lane & 15;
-    const int cg = blockIdx.x % cgroups, rg = blockIdx.x / cgroups;
-    const int tile = wave_rows ? rg * kExpandWaves + wave : rg;
+//
+// A tile's work is its distinct adapters (rows with none, where there is
+// something to do for them, count as one more) times the blocks of columns,
+// adapter by adapter; `share` work-groups split it evenly into runs of at
+// least nblocks.  How many adapters a tile names is known here only: one for
+// most tiles of a prompt, dozens for sequences decoding together.
+template <bool GLU, int MC, bool BB>
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(MC > 2 ? 2 : 4))) void lora_expand_kernel(
+    LoraArgs p, int splits, int share, int nblocks) {
+    constexpr int kMaxPitch = (MC == 0 ? 2 : MC == 1 ? 4 : 8) + 1;
+    __shared__ u32x4 lds[2 * 64 * kMaxPitch];
+    const int wave = threadIdx.x / kWave, lane = threadIdx.x & (kWave - 1);
+    // part by part over the tiles, the last ones first: those that a tile of
+    // one adapter leaves unused end at once, on every XCD alike, and those of
+    // tiles of two start before the others
+    const int tiles = gridDim.x / share, part = share - 1 - blockIdx.x / tiles, tile = blockIdx.x % tiles;
+    constexpr int kBlock = GLU ? 32 : 64;
     const int width = GLU ? p.N / 2 : p.N;                 // columns of y
-    const int first = (wave_rows ? cg : cg * kExpandWaves + wave) * ngroups * G * kCols;
-    const int last = min(width, first + ngroups * G * kCols);
-    const int item = blockIdx.y;
-    if (tile * kRows >= p.T || first >= width) return;
-    const Tile t = tile_rows(p, tile);
-    // rows without an adapter are a group of their own (slot -1): they copy
-    // base, which in place is nothing to do
+    const int blocks = (width + kBlock - 1) / kBlock;
+    const Tile t = tile_rows<kExpandRows>(p, tile);
+    const int64_t row0 = int64_t(tile) * kExpandRows + wave * kRows;
+    // rows without an adapter copy base, which in place is nothing to do
     const bool copy = GLU || p.base != p.y;
-    uint64_t todo = (copy ? __ballot(t.in) : __ballot(t.slot >= 0)) & 0xFFFFu;
-    for (int it = 0; todo; ++it) {
+    uint64_t todo = copy ? __ballot(t.in) : __ballot(t.slot >= 0);
+    int count = 0, slots = 0;                              // lane i: the i-th distinct adapter
+    while (todo) {
         int lead;
         const int slot = next_slot(t, todo, lead);
-        if (items > 1 && it != item) continue;
-        const bool mine = t.in && t.slot == slot;
-        const int lead_row = __builtin_amdgcn_readlane(t.row, lead);
+        slots = lane == count ? slot : slots;
+        ++count;
+    }
+    const int64_t total = int64_t(count) * blocks;
+    const int64_t run = max(int64_t(nblocks), (total + share - 1) / share);
+    int64_t at = part * run;
+    const int64_t end = min(total, at + run);
+    while (at < end) {
+        const int g = int(at / blocks), b0 = int(at - int64_t(g) * blocks);
+        const int n = int(min(end - at, int64_t(blocks - b0)));
+        at += n;
+        const int first = b0 * kBlock, last = min(width, first + n * kBlock);
+        const int slot = __builtin_amdgcn_readlane(slots, g);
+        const uint32_t mask = uint32_t(__ballot(t.in && t.slot == slot) >> (wave * kRows)) & 0xFFFFu;
         const int rank = slot < 0 ? 0 : min(max(p.rank[slot], 0), p.R);
 #define GRIM_COLS(CC, HALF) \
-    expand_cols<GLU, CC, HALF, BB, G>(p, splits, slot, rank, t.row, lead_row, mine, q, col, first, last, width)
+    expand_cols<GLU, CC, HALF, BB>(p, splits, slot, rank, mask, row0, first, last, width, lds)
         if (rank == 0) {
             if (copy) GRIM_COLS(0, false);
         } else if constexpr (MC == 0) {
@@ -430,14 +545,13 @@ __global__ __launch_bounds__(kExpandWaves * kWave) void lora_expand_kernel(LoraA
             else GRIM_COLS(MC, false);
         }
 #undef GRIM_COLS
-        if (items > 1) break;
     }
 }
 
-// K splits over work-groups: as many as leave each wave two steps, for short
+// K splits over work-groups: as many as leave each wave one step, for short
 // batches; long ones take as many of these as make two work-groups a CU.
 int short_splits(int K) {
-    const int ksteps = (K + kStep - 1) / kStep, s = (ksteps + 2 * kShrinkWaves - 1) / (2 * kShrinkWaves);
+    const int ksteps = (K + kStep - 1) / kStep, s = (ksteps + kShrinkWaves - 1) / kShrinkWaves;
     return s > kMaxSplits ? kMaxSplits : s;
 }
 constexpr int kShrinkGroups = 512;
@@ -463,42 +577,32 @@ void shrink(hipStream_t st, const LoraArgs& a, int splits, int items) {
 #undef GRIM_SHRINK
 }
 
-constexpr int kExpandWavesBusy = 4096;   // waves that fill the chip: 16 a CU
-
-template <bool GLU, int MC, bool BB, int G>
-void expand_g(hipStream_t st, const LoraArgs& a, int splits, int items, int64_t waves) {
-    const int tiles = (a.T + kRows - 1) / kRows;
-    const int width = GLU ? a.N / 2 : a.N, groups = (width + G * kCols - 1) / (G * kCols);
-    // a work-group's waves: four row tiles of the same columns, which share
-    // B's rows in the L1 (long batches), or four column ranges of one tile;
-    // columns of a wave so that the chip is filled about once
-    const int wave_rows = a.T > kItemRows;
-    int ng = int(waves / G / kExpandWavesBusy);
-    ng = ng < 1 ? 1 : ng > groups ? groups : ng;
-    const int per = ng * (wave_rows ? 1 : kExpandWaves), cgroups = (groups + per - 1) / per;
-    const int rgroups = wave_rows ? (tiles + kExpandWaves - 1) / kExpandWaves : tiles;
-    hipLaunchKernelGGL((lora_expand_kernel<GLU, MC, BB, G>), dim3(unsigned(cgroups) * rgroups, items),
-                       dim3(kExpandWaves * kWave), 0, st, a, splits, items, wave_rows, cgroups, ng);
-}
+// expand's work-groups, 4 a CU at once: runs of blocks of two of them while
+// every tile is one adapter's, which leaves room for the tiles of two (4096
+// rows of 9 requests, 2048 -> 7168: 34.8 us; runs that fill the chip: 40.4);
+// three of them share out tiles of many (48 mixed rows of 32 adapters:
+// 12.2 us against 15 with two or four).
+constexpr int kExpandRuns = 512, kExpandGroups = 768;
 
 template <bool GLU, bool BB>
-void expand(hipStream_t st, const LoraArgs& a, int splits, int items) {
-    const int width = GLU ? a.N / 2 : a.N;
-    constexpr int G = GLU ? 2 : 4;
-    // waves of one block each (every row tile with as many adapters as it
-    // can name); fewer than fill the chip stay at one block
-    const int64_t waves = int64_t((a.T + kRows - 1) / kRows) * items * ((width + kCols - 1) / kCols);
-    const bool one = waves < kExpandWavesBusy * G;
-#define GRIM_EXPAND(MC)                                                              \
-    do {                                                                             \
-        if (one) expand_g<GLU, MC, BB, 1>(st, a, splits, items, waves);              \
-        else expand_g<GLU, MC, BB, G>(st, a, splits, items, waves);                  \
-    } while (0)
+void expand(hipStream_t st, const LoraArgs& a, int splits) {
+    const int tiles = (a.T + kExpandRows - 1) / kExpandRows;
+    const int width = GLU ? a.N / 2 : a.N, block = GLU ? 32 : 64, blocks = (width + block - 1) / block;
+    // twice the work-groups that tiles of one adapter need, so that tiles of
+    // two take no longer (the others' second half ends at once)
+    const int nb = int((int64_t(tiles) * blocks + kExpandRuns - 1) / kExpandRuns);
+    int64_t share = 2 * ((blocks + nb - 1) / nb);
+    if (share < kExpandGroups / tiles) share = kExpandGroups / tiles;
+    const int64_t most = int64_t(a.T < kExpandRows ? a.T : kExpandRows) * blocks;
+    if (share > most) share = most;
+    const dim3 grid(unsigned(share) * tiles);
+#define GRIM_EXPAND(MC) \
+    hipLaunchKernelGGL((lora_expand_kernel<GLU, MC, BB>), grid, dim3(kThreads), 0, st, a, splits, int(share), nb)
     if (a.R <= 16) GRIM_EXPAND(0);
     else if (a.R <= 32) GRIM_EXPAND(1);
     else if (a.R <= 64) GRIM_EXPAND(2);
-    else if (a.R <= 128) expand_g<GLU, 4, BB, 1>(st, a, splits, items, waves);
-    else expand_g<GLU, 8, BB, 1>(st, a, splits, items, waves);
+    else if (a.R <= 128) GRIM_EXPAND(4);
+    else GRIM_EXPAND(8);
 #undef GRIM_EXPAND
 }
 
@@ -507,8 +611,9 @@ void expand(hipStream_t st, const LoraArgs& a, int splits, int items) {
 size_t lora_workspace_bytes(int K, int R, int T) {
     if (K <= 0 || R <= 0 || T <= 0) return 0;
     // for up to T rows: splits * rows is at most this for every shorter batch
-    const size_t most = size_t(short_splits(K)) * T, lng = size_t(kShrinkGroups) * kRows + T;
-    return (most < lng || T <= kItemRows ? most : lng) * R * sizeof(float);
+    const size_t rows = (size_t(T) + kRows - 1) / kRows * kRows, most = short_splits(K) * rows;
+    const size_t lng = size_t(kShrinkGroups) * kRows + rows;
+    return (most < lng || T <= kItemRows ? most : lng) * ((R + 31) / 32 * 32) * sizeof(float);
 }
 
 hipError_t lora_launch(hipStream_t st, const LoraArgs& a) {
@@ -520,8 +625,8 @@ hipError_t lora_launch(hipStream_t st, const LoraArgs& a) {
     else shrink<false>(st, a, splits, items);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    if (a.glu) a.base_bf16 ? expand<true, true>(st, a, splits, items) : expand<true, false>(st, a, splits, items);
-    else a.base_bf16 ? expand<false, true>(st, a, splits, items) : expand<false, false>(st, a, splits, items);
+    if (a.glu) a.base_bf16 ? expand<true, true>(st, a, splits) : expand<true, false>(st, a, splits);
+    else a.base_bf16 ? expand<false, true>(st, a, splits) : expand<false, false>(st, a, splits);
     return hipGetLastError();
 }
 

@@ -20,10 +20,11 @@ struct LoraArgs {
     int64_t x_stride, base_stride, y_stride;
     int x_bf16, base_bf16, y_bf16;
     int T, glu;
-    float* part;              // workspace: [splits][T][R] partials of A x
+    float* part;              // workspace: partials of A x by K split
 };
 
 constexpr int kLoraMaxRank = 256;
+constexpr int64_t kLoraMaxStride = int64_t(1) << 24;
 
 size_t lora_workspace_bytes(int K, int R, int T);
 hipError_t lora_launch(hipStream_t st, const LoraArgs& a);

@@ -428,7 +428,7 @@ size_t grimoire_lora_workspace_bytes(const grim_lora* L, int rows);
 /* y[t] = base[t] + scale_a B_a (A_a x[t]); rows without an adapter are
  * copied (in place: left as they are).  x [rows][K], base and y [rows][N]:
  * fp32 or bf16 rows, *_stride elements apart (x a multiple of 8, base and y
- * of 4); fp32 and x rows 16-byte, bf16 base and y rows 8-byte aligned.  y may
+ * of 4; at most 2^24), max_rank * K and max_rank * N at most 2^29; fp32 and x rows 16-byte, bf16 base and y rows 8-byte aligned.  y may
  * be base (same type and stride) and overlaps nothing else.  Sums are fp32,
  * in an order that does not depend on the other rows' adapters; fp32
  * activations are multiplied in full precision. */

@@ -90,6 +90,9 @@ def lora(glu=False, rows=3, slot=A, x=A, x_bf16=0, x_stride=64, base=A, base_bf1
     (dict(base=A + 4, base_bf16=1), ARG), (dict(y=A + 8), ARG), (dict(a=A + 8), ARG), (dict(b=A + 2), ARG),
     (dict(y=A, y_bf16=1), ARG), (dict(y=A, y_stride=36), ARG), (dict(glu=True, y=A), ARG),
     (dict(glu=True, N=36, base_stride=36), SHAPE), (dict(glu=True, y_stride=12), SHAPE),
+    (dict(x_stride=(1 << 24) + 8), SHAPE), (dict(base_stride=(1 << 24) + 4), SHAPE),
+    (dict(y_stride=(1 << 24) + 4), SHAPE), (dict(K=1 << 22, x_stride=1 << 22, max_rank=256), SHAPE),
+    (dict(N=1 << 22, base_stride=1 << 22, y_stride=1 << 22, max_rank=256), SHAPE),
     (dict(ws=None), _abi.ERR_WORKSPACE), (dict(ws_bytes=3 * 16 * 4 - 1), _abi.ERR_WORKSPACE), (dict(ws=A + 4), ARG)])
 def test_lora(kw, status):
     assert lora(**kw) == status
