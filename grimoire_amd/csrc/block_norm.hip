@@ -6,9 +6,13 @@
 // Two dependent sums over a row, so the row stays in registers: thread i of
 // a work-group holds the 4-column chunks i, i + NT, ...  Memory bound: h and
 // f are read once, h', o written once.  Everything the row needs (h, gate,
-// weights) is requested before the first barrier, so one memory latency is
-// paid a row and not three.  Sums are fp32 over at most 32 squares a thread,
-// then a tree.
+// weights, expert rows) is requested before the first barrier and without a
+// branch in between, so one memory latency is paid a row and not three.  Sums
+// are fp32 over at most 32 squares a thread, then a tree.
+//
+// 4096 x 7168, bf16 block output, bf16 gate an element: 98.6 us, 5.4 TB/s
+// (a large copy: 4.94); 3001 x 2048 behind ten experts and a shared one: 48.2
+// us, 4.9 TB/s.  One to 32 rows: 3 to 7 us, two barriers and a chain of loads.
 #include "block_norm.hpp"
 
 namespace grim {
@@ -58,57 +62,84 @@ __global__ __launch_bounds__(NT) void block_norm_kernel(BlockNormArgs a) {
     const int64_t base = t * H;
     __shared__ float part[2][NT / kWave];
 
+    // No load below waits for a branch: columns past H read the row's last
+    // four, routes without a row here and absent weights read the row of h,
+    // and what was read for nothing is left out of the arithmetic.
+    const float* hrow = a.h + base;
+    const uint16_t* dummy = reinterpret_cast<const uint16_t*>(hrow);
     const uint16_t* rrow[KT > 0 ? KT : 1];
     float rw[KT > 0 ? KT : 1];
+    bool on[KT > 0 ? KT : 1];
     if constexpr (KT > 0) {
 #pragma unroll
         for (int s = 0; s < KT; ++s) {
-            int p = s < a.K ? a.inverse[t * a.K + s] : -1;
-            p = p < a.routed_rows ? p : -1;
-            rrow[s] = p < 0 ? nullptr : a.routed + int64_t(p) * H;
-            rw[s] = p < 0 ? 0.0f : a.rw[t * a.K + s];
+            const int64_t r = t * a.K + (s < a.K ? s : a.K - 1);
+            const int p = a.inverse[r];
+            on[s] = s < a.K && p >= 0 && p < a.routed_rows;
+            rrow[s] = on[s] ? a.routed + int64_t(p) * H : dummy;
+            rw[s] = a.rw[r];
         }
     }
-    float row_gate = 1.0f;
-    if (a.gate_kind == GRIM_GATE_ROW)
-        row_gate = a.gate_bf16 ? bf16_to_f32(static_cast<const uint16_t*>(a.gate)[t])
-                               : static_cast<const float*>(a.gate)[t];
-
-    F4 f[VPT], h[VPT], g[VPT];
-    uint2 wp[VPT], wn[VPT];
+    int d[VPT];
+    bool in[VPT];
 #pragma unroll
     for (int c = 0; c < VPT; ++c) {
-        const int d = (int(threadIdx.x) + c * NT) * 4;
-        if (d >= H) continue;
-        if constexpr (SRC == kSrcF32) {
-            f[c] = load_f32(static_cast<const float*>(a.x) + t * a.x_stride + d);
-        } else if constexpr (SRC == kSrcBf16) {
-            f[c] = load_b16(static_cast<const uint16_t*>(a.x) + t * a.x_stride + d);
-        } else {
-            // a route without a row here adds nothing (its row is not read)
-            f[c] = a.shared ? load_f32(a.shared + base + d) : F4{{0.0f, 0.0f, 0.0f, 0.0f}};
-            uint2 u[KT > 0 ? KT : 1];
+        const int o = (int(threadIdx.x) + c * NT) * 4;
+        in[c] = o < H;
+        d[c] = in[c] ? o : H - 4;
+    }
+
+    constexpr bool kAhead = VPT <= 4;      // weights too, where the registers hold them
+    F4 f[VPT], h[VPT], g[VPT];
+    uint2 wp[kAhead ? VPT : 1], wn[kAhead ? VPT : 1];
+    const uint16_t* post = a.post_w ? a.post_w : dummy;
+    const uint16_t* pre = a.pre_w ? a.pre_w : dummy;
 #pragma unroll
-            for (int s = 0; s < KT; ++s)
-                u[s] = rrow[s] ? *reinterpret_cast<const uint2*>(rrow[s] + d) : make_uint2(0u, 0u);
+    for (int c = 0; c < VPT; ++c) {
+        h[c] = load_f32(hrow + d[c]);
+        if constexpr (kAhead) {
+            wp[c] = *reinterpret_cast<const uint2*>(post + d[c]);
+            wn[c] = *reinterpret_cast<const uint2*>(pre + d[c]);
+        }
+        if constexpr (SRC == kSrcF32) f[c] = load_f32(static_cast<const float*>(a.x) + t * a.x_stride + d[c]);
+        if constexpr (SRC == kSrcBf16) f[c] = load_b16(static_cast<const uint16_t*>(a.x) + t * a.x_stride + d[c]);
+    }
+    if (a.gate_kind == GRIM_GATE_CHANNEL || a.gate_kind == GRIM_GATE_FULL) {
+        const int64_t o = a.gate_kind == GRIM_GATE_FULL ? base : 0;
+        if (a.gate_bf16) {
+#pragma unroll
+            for (int c = 0; c < VPT; ++c) g[c] = load_b16(static_cast<const uint16_t*>(a.gate) + o + d[c]);
+        } else {
+#pragma unroll
+            for (int c = 0; c < VPT; ++c) g[c] = load_f32(static_cast<const float*>(a.gate) + o + d[c]);
+        }
+    } else {
+        float row_gate = 1.0f;
+        if (a.gate_kind == GRIM_GATE_ROW)
+            row_gate = a.gate_bf16 ? bf16_to_f32(static_cast<const uint16_t*>(a.gate)[t])
+                                   : static_cast<const float*>(a.gate)[t];
+#pragma unroll
+        for (int c = 0; c < VPT; ++c) g[c] = F4{{row_gate, row_gate, row_gate, row_gate}};
+    }
+    if constexpr (KT > 0) {
+#pragma unroll
+        for (int c = 0; c < VPT; ++c) f[c] = F4{{0.0f, 0.0f, 0.0f, 0.0f}};
+        if (a.shared) {
+#pragma unroll
+            for (int c = 0; c < VPT; ++c) f[c] = load_f32(a.shared + base + d[c]);
+        }
+#pragma unroll
+        for (int c = 0; c < VPT; ++c) {
+            uint2 u[KT];
+#pragma unroll
+            for (int s = 0; s < KT; ++s) u[s] = *reinterpret_cast<const uint2*>(rrow[s] + d[c]);
 #pragma unroll
             for (int s = 0; s < KT; ++s) {
                 const F4 e = widen(u[s]);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) f[c].v[i] = __builtin_fmaf(rw[s], e.v[i], f[c].v[i]);
+                for (int i = 0; i < 4; ++i) f[c].v[i] = on[s] ? __builtin_fmaf(rw[s], e.v[i], f[c].v[i]) : f[c].v[i];
             }
         }
-        h[c] = load_f32(a.h + base + d);
-        if (a.gate_kind >= GRIM_GATE_CHANNEL && a.gate_kind != GRIM_GATE_ROW) {
-            const int64_t o = (a.gate_kind == GRIM_GATE_FULL ? base : 0) + d;
-            g[c] = a.gate_bf16 ? load_b16(static_cast<const uint16_t*>(a.gate) + o)
-                               : load_f32(static_cast<const float*>(a.gate) + o);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) g[c].v[i] = row_gate;
-        }
-        wp[c] = a.post_w ? *reinterpret_cast<const uint2*>(a.post_w + d) : make_uint2(0u, 0u);
-        wn[c] = a.pre_w ? *reinterpret_cast<const uint2*>(a.pre_w + d) : make_uint2(0u, 0u);
     }
 
     float fs = 1.0f;
@@ -116,9 +147,10 @@ __global__ __launch_bounds__(NT) void block_norm_kernel(BlockNormArgs a) {
         float ss = 0.0f;
 #pragma unroll
         for (int c = 0; c < VPT; ++c) {
-            if ((int(threadIdx.x) + c * NT) * 4 >= H) continue;
+            float q = ss;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) ss = __builtin_fmaf(f[c].v[i], f[c].v[i], ss);
+            for (int i = 0; i < 4; ++i) q = __builtin_fmaf(f[c].v[i], f[c].v[i], q);
+            ss = in[c] ? q : ss;
         }
         fs = rsqrtf(block_sum<NT>(ss, part[0]) / float(H) + a.eps);
     }
@@ -126,36 +158,35 @@ __global__ __launch_bounds__(NT) void block_norm_kernel(BlockNormArgs a) {
     float ss = 0.0f;
 #pragma unroll
     for (int c = 0; c < VPT; ++c) {
-        const int d = (int(threadIdx.x) + c * NT) * 4;
-        if (d >= H) continue;
-        const F4 w = widen(wp[c]);
+        const F4 w = kAhead ? widen(wp[kAhead ? c : 0]) : load_b16(post + d[c]);
+        float s = ss;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             float p = f[c].v[i];
             if (a.post_w) p = p * fs * (a.offset + w.v[i]);
             p *= gate_act(g[c].v[i], act);
             h[c].v[i] = __builtin_fmaf(a.bs, p, a.rs * h[c].v[i]);
-            ss = __builtin_fmaf(h[c].v[i], h[c].v[i], ss);
+            s = __builtin_fmaf(h[c].v[i], h[c].v[i], s);
         }
-        if (a.h_out)
-            *reinterpret_cast<float4*>(a.h_out + base + d) = make_float4(h[c].v[0], h[c].v[1], h[c].v[2], h[c].v[3]);
+        ss = in[c] ? s : ss;
+        if (a.h_out && in[c])
+            *reinterpret_cast<float4*>(a.h_out + base + d[c]) = make_float4(h[c].v[0], h[c].v[1], h[c].v[2], h[c].v[3]);
     }
     if (!a.out && !a.out_bf) return;
     const float hs = rsqrtf(block_sum<NT>(ss, part[1]) / float(H) + a.eps);
 #pragma unroll
     for (int c = 0; c < VPT; ++c) {
-        const int d = (int(threadIdx.x) + c * NT) * 4;
-        if (d >= H) continue;
-        const F4 w = widen(wn[c]);
+        if (!in[c]) continue;
+        const F4 w = kAhead ? widen(wn[kAhead ? c : 0]) : load_b16(pre + d[c]);
         float o[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) o[i] = h[c].v[i] * hs * (a.offset + w.v[i]);
-        if (a.out) *reinterpret_cast<float4*>(a.out + base + d) = make_float4(o[0], o[1], o[2], o[3]);
+        if (a.out) *reinterpret_cast<float4*>(a.out + base + d[c]) = make_float4(o[0], o[1], o[2], o[3]);
         if (a.out_bf) {
             uint2 b;
             b.x = uint32_t(f32_to_bf16(o[0])) | (uint32_t(f32_to_bf16(o[1])) << 16);
             b.y = uint32_t(f32_to_bf16(o[2])) | (uint32_t(f32_to_bf16(o[3])) << 16);
-            *reinterpret_cast<uint2*>(a.out_bf + base + d) = b;
+            *reinterpret_cast<uint2*>(a.out_bf + base + d[c]) = b;
         }
     }
 }
@@ -168,6 +199,7 @@ void launch_src(hipStream_t st, const BlockNormArgs& a) {
         else GRIM_BN(kSrcF32);
     } else if (a.K <= 2) GRIM_BN(2 + 2);
     else if (a.K <= 4) GRIM_BN(2 + 4);
+    else if (a.K <= 6) GRIM_BN(2 + 6);
     else if (a.K <= 8) GRIM_BN(2 + 8);
     else if (a.K <= 10) GRIM_BN(2 + 10);
     else GRIM_BN(2 + 16);
@@ -176,12 +208,23 @@ void launch_src(hipStream_t st, const BlockNormArgs& a) {
 
 }  // namespace
 
+// Up to this many rows (one a CU) a row is spread over 1024 threads rather
+// than 256 or 512 with more columns each: 8 rows of 2880, 3.50 against 3.82
+// us; 32 of 2048 behind ten experts, 4.28 against 4.45; 512 of 7168 behind
+// eight, 30.6 against 28.3.
+constexpr int kFewRows = 256;
+
 hipError_t block_norm_launch(hipStream_t st, const BlockNormArgs& a) {
     if (a.T <= 0) return hipSuccess;
     if (a.H <= 0 || a.H % 4 || a.H > kBlockNormMaxHidden || a.K < 0 || a.K > 16) return hipErrorInvalidValue;
     const int chunks = a.H / 4;
+    // few rows: a row's loads over as many waves as a CU holds
+    const bool few = a.T <= kFewRows;
     if (chunks <= 64) launch_src<64, 1>(st, a);
     else if (chunks <= 256) launch_src<256, 1>(st, a);
+    else if (few && chunks <= 512) launch_src<512, 1>(st, a);
+    else if (few && chunks <= 1024) launch_src<1024, 1>(st, a);
+    else if (few && chunks <= 2048) launch_src<1024, 2>(st, a);
     else if (chunks <= 512) launch_src<256, 2>(st, a);
     else if (chunks <= 1024) launch_src<256, 4>(st, a);
     else if (chunks <= 2048) launch_src<512, 4>(st, a);

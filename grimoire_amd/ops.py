@@ -334,6 +334,13 @@ def _flat(t: Optional[torch.Tensor], what: str, shape, dtypes, dev: int):
     return t.data_ptr()
 
 
+def _gpu(t: torch.Tensor) -> int:
+    dev = t.get_device()
+    if dev < 0:
+        _dev(t)
+    return dev
+
+
 def _launch(dev: int, stream, fn, what: str, *args):
     """Call entry point fn(stream, *args) with device dev current and check
     its status; stream None: dev's current stream."""
@@ -368,22 +375,23 @@ class RouteScores:
         self.bias = bias
         self.struct = _abi.ScoreParams(self.SCORES[score], n_group, topk_group, self.GROUPS[group_score],
                                        int(normalize), float(scaling), _p(bias))
+        self._bias_of = None if bias is None else (bias.numel(), bias.get_device())
+        self._call = lib().grimoire_moe_router_scores
+        self._ref = C.byref(self.struct)
 
     def __call__(self, logits, out_expert, out_weight, stream=None):
         """Routes of logits [T][E] (fp32 or bf16, rows may lie apart) into
         out_expert int32 / out_weight fp32 [T][K]."""
-        _dev(logits)
-        dev = logits.get_device()
+        dev = _gpu(logits)
         if out_expert.dim() != 2 or logits.dim() != 2:
             raise _abi.GrimoireError("logits [T][E], out_expert [T][K]")
-        T, K = out_expert.shape
+        T, K = shape = out_expert.shape
         E = logits.shape[1]
         lp, b16, stride = _rows(logits, "logits", E, T)
-        if self.bias is not None and (self.bias.numel() != E or self.bias.get_device() != dev):
+        if self._bias_of is not None and self._bias_of != (E, dev):
             raise _abi.GrimoireError("bias: one value an expert, on the logits' device")
-        _launch(dev, stream, lib().grimoire_moe_router_scores, "router_scores", self.struct, lp, b16, stride, T, E,
-                K, _flat(out_expert, "out_expert", (T, K), _I32, dev),
-                _flat(out_weight, "out_weight", (T, K), _F32, dev))
+        _launch(dev, stream, self._call, "router_scores", self._ref, lp, b16, stride, T, E, K,
+                _flat(out_expert, "out_expert", shape, _I32, dev), _flat(out_weight, "out_weight", shape, _F32, dev))
 
 
 class BlockNorm:
@@ -403,25 +411,26 @@ class BlockNorm:
                 _dev(w)
                 _flat(w, "norm weight", (w.numel(),), _B16, w.get_device())
         self.pre_weight, self.post_weight, self.gate = pre_weight, post_weight, gate
+        self._weights_of = {(w.numel(), w.get_device()) for w in (pre_weight, post_weight) if w is not None}
+        self._dense, self._moe = lib().grimoire_block_norm, lib().grimoire_moe_block_norm
         self.struct = _abi.BlockNormParams(_p(post_weight), _p(pre_weight), float(weight_offset), float(eps),
                                            float(residual_scale), float(block_scale), self.GATES[gate],
                                            int(gate_sigmoid))
+        self._ref = C.byref(self.struct)
 
     def _args(self, h, h_out, out, out_bf, gate):
-        _dev(h)
-        dev = h.get_device()
-        T, H = h.shape
-        for w in (self.pre_weight, self.post_weight):
-            if w is not None and (w.numel() != H or w.get_device() != dev):
+        dev = _gpu(h)
+        T, H = shape = h.shape
+        for of in self._weights_of:
+            if of != (H, dev):
                 raise _abi.GrimoireError("norm weights: one value a column, on h's device")
         kind = self.gate
         if (gate is not None) != (kind != "none"):
             raise _abi.GrimoireError(f"gate {kind!r} and the gate tensor do not go together")
         gp, g16 = None, 0
         if gate is not None:
-            gp = _flat(gate, "gate", (H,) if kind == "channel" else (T,) if kind == "row" else (T, H), _FB16, dev)
-            g16 = int(gate.dtype is not torch.float32)
-        shape = (T, H)
+            gp = _flat(gate, "gate", (H,) if kind == "channel" else (T,) if kind == "row" else shape, _FB16, dev)
+            g16 = gate.dtype is not _f32
         return (T, H, dev, gp, g16, _flat(h, "h", shape, _F32, dev), _flat(h_out, "h_out", shape, _F32, dev),
                 _flat(out, "out", shape, _F32, dev), _flat(out_bf, "out_bf", shape, _B16, dev))
 
@@ -431,8 +440,7 @@ class BlockNorm:
         xp, x16, stride = _rows(x, "x", H, T)
         if x.get_device() != dev:
             raise _abi.GrimoireError("x: on another device than h")
-        _launch(dev, stream, lib().grimoire_block_norm, "block_norm", self.struct, gp, g16, hp, xp, x16, stride, hop, op,
-                obp, T, H)
+        _launch(dev, stream, self._dense, "block_norm", self._ref, gp, g16, hp, xp, x16, stride, hop, op, obp, T, H)
 
     def moe(self, h, routed, inverse, route_weight, shared, h_out, out=None, out_bf=None, gate=None, stream=None):
         """Behind routed experts (grimoire_moe_block_norm): routed bf16
@@ -441,7 +449,7 @@ class BlockNorm:
         if route_weight.dim() != 2:
             raise _abi.GrimoireError("route_weight: [T][K]")
         K = route_weight.shape[1]
-        _launch(dev, stream, lib().grimoire_moe_block_norm, "moe_block_norm", self.struct, gp, g16, hp,
+        _launch(dev, stream, self._moe, "moe_block_norm", self._ref, gp, g16, hp,
                 _flat(routed, "routed", (routed.shape[0], H), _B16, dev), routed.shape[0],
                 _flat(inverse.view(-1), "inverse", (T * K,), _I32, dev),
                 _flat(route_weight, "route_weight", (T, K), _F32, dev), _flat(shared, "shared", (T, H), _F32, dev), hop,
@@ -463,9 +471,11 @@ class Lora:
         self.dev = adapters.a.get_device()
         nbytes = int(lib().grimoire_lora_workspace_bytes(self.struct, max_rows))
         self.workspace = torch.empty(nbytes, dtype=torch.uint8, device=adapters.a.device)
+        self._ref = C.byref(self.struct)
+        self._add, self._swiglu = lib().grimoire_lora_add, lib().grimoire_lora_swiglu
 
     def _call(self, fn, what, row_slot, x, base, y, width, stream):
-        _dev(x)
+        _gpu(x)
         A, dev = self.adapters, self.dev
         T = x.shape[0]
         if T > self.max_rows:
@@ -475,20 +485,20 @@ class Lora:
         xp, x16, xs = _rows(x, "x", A.K, T)
         bp, b16, bs = _rows(base, "base", A.N, T)
         yp, y16, ys = _rows(y, "output", width, T)
-        _launch(dev, stream, fn, what, self.struct, _flat(row_slot, "row_slot", (T,), _I32, dev), xp, x16, xs, bp, b16,
+        _launch(dev, stream, fn, what, self._ref, _flat(row_slot, "row_slot", (T,), _I32, dev), xp, x16, xs, bp, b16,
                 bs, yp, y16, ys, T, self.workspace.data_ptr(), self.workspace.numel())
 
     def add(self, row_slot, x, y, base=None, stream=None):
         """y = base + the adapters' product of x (base None: y += it).
         row_slot int32 [T]; x [T][K], base and y [T][N] fp32 or bf16, rows
         may lie apart."""
-        self._call(lib().grimoire_lora_add, "lora_add", row_slot, x, y if base is None else base, y, self.adapters.N,
+        self._call(self._add, "lora_add", row_slot, x, y if base is None else base, y, self.adapters.N,
                    stream)
 
     def swiglu(self, row_slot, x, base, h, stream=None):
         """h [T][N/2] = silu(gate) * up of the gate|up projection base
         [T][N] plus the adapters' product of x."""
-        self._call(lib().grimoire_lora_swiglu, "lora_swiglu", row_slot, x, base, h, self.adapters.N // 2, stream)
+        self._call(self._swiglu, "lora_swiglu", row_slot, x, base, h, self.adapters.N // 2, stream)
 
 
 # ------------------------------------------------------------------- layer
