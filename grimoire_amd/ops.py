@@ -461,7 +461,8 @@ class BlockNorm:
 class Lora:
     """Low-rank adapters of many requests beside one shared projection
     (grimoire_lora_add / grimoire_lora_swiglu), with the workspace of up to
-    max_rows rows."""
+    max_rows rows: calls of one object must not overlap.  What changes in the
+    adapters' tensors (`LoraAdapters.load`) holds for the next call."""
 
     def __init__(self, adapters: LoraAdapters, max_rows: int):
         _dev(adapters.a)

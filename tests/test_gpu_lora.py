@@ -167,6 +167,21 @@ def test_a_row_does_not_depend_on_the_others(gpu, T, order):
     z = run(e, gpu)
     assert torch.equal(y[keep], z[keep])
     assert torch.equal(run(d, gpu), y)
+    # an adapter of NaNs is its own rows' matter too
+    n = dict(d, a=d["a"].clone(), b=d["b"].clone(), scale=d["scale"].clone())
+    n["a"][2], n["b"][2], n["scale"][2] = float("nan"), float("inf"), float("nan")
+    z = run(n, gpu)
+    assert torch.equal(y[d["slot"] != 2], z[d["slot"] != 2])
+
+
+def test_full_ranks_and_many_adapters_in_a_tile(gpu):
+    """64 adapters in the 64 rows of a tile, each rank of the storage."""
+    for R in (16, 32, 48, 64, 80, 128, 256):
+        d = make(130, 72, 72, 64, R, R, ranks=[(7 * i) % R + 1 for i in range(64)])
+        d["slot"] = torch.randperm(130, generator=gen(R)).remainder(64).int()
+        check(d, gpu)
+        check(d, gpu, glu=True)
+        check(dict(d, slot=d["slot"].sort().values), gpu, inplace=True)
 
 
 def test_large_and_tiny_values(gpu):

@@ -24,6 +24,8 @@ CASES = [  # regime, name, T, E, K, H, I, fmt, n_group, topk_group, shared
     (5, "grouped_valu", 12, 64, 8, 512, 512, "int4", 1, 1, False),
     (0, "wreg", 60, 32, 4, 512, 256, "bf16", 1, 1, False),
     (0, "prompt", 520, 32, 4, 512, 256, "int8", 4, 2, False),
+    # the split-K router leaves two partial sums: the scores kernel adds them
+    (0, "split_router", 4200, 64, 4, 512, 128, "int8", 1, 1, False),
 ]
 
 

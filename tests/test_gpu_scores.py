@@ -107,6 +107,8 @@ def test_ties_and_borders(gpu, score):
     l = rand(64, 200, 4).round()
     check(gpu, l, 12, score=score)
     check(gpu, l, 9, score=score, n_group=10, topk_group=3, group_score="top2")
+    check(gpu, torch.zeros(3, 512), 16, score=score)              # more ties than lanes
+    check(gpu, torch.zeros(3, 512), 16, score=score, n_group=64, topk_group=9)
     near = torch.full((4, 96), 0.75)
     near[:, 50] = torch.nextafter(near[0, 0], torch.tensor(1.0))
     near[:, 20] = torch.nextafter(near[0, 0], torch.tensor(0.0))
