@@ -1,9 +1,10 @@
 // lora.hip -- low-rank adapters of many requests beside a shared projection:
 //   y_t = base_t + scale_a B_a (A_a x_t),  a = row_slot[t]
-// in two launches.  shrink: z_t = A_a x_t, K split over waves and
-// work-groups, fp32 partials to the workspace.  expand: the partials are
-// summed in a fixed order, scaled, multiplied with B_a and added to base
-// (and, for a gate|up projection, SwiGLU'd) on the way to y.
+// in two launches (one for a few rows of small adapters).  shrink: z_t =
+// A_a x_t, K split over waves and work-groups, fp32 partials to the
+// workspace.  expand: the partials are summed in a fixed order, scaled,
+// multiplied with B_a and added to base (and, for a gate|up projection,
+// SwiGLU'd) on the way to y.
 //
 // Both are memory bound at every size (2 r operations an element of x and y
 // read or written), and their rows go through the LDS on the way to the
@@ -15,8 +16,8 @@
 // TB/s of a large copy): 4096 rows of 9 requests, 2048 -> 7168, rank 64 of
 // mixed ranks, bf16: 13 + 35 (28; base copied to y by the same loop 25.5);
 // 2001 rows of 5, 2880 -> 2 x 2880, rank 16, fp32: 11 + 19 (19); 48 mixed
-// rows of 32 adapters, 2048 -> 7168: 6 + 12 (3.3); one row: 4 + 5, two
-// dependent chains of loads.
+// rows of 32 adapters, 2048 -> 7168: 6 + 12 (3.3); one row, 768 -> 2048: 5 in
+// one launch, a chain of dependent loads.
 //
 // fp32 values are multiplied exactly: an fp32 x (and z) is the sum of three
 // bf16 pieces of 8 significant bits, cut off, not rounded, so each rest is
@@ -313,7 +314,6 @@ __device__ __forceinline__ void store_cols(void* y, uint32_t off, int bf16, cons
 // ranks, an odd number of pieces: the 16 rows of a tile's read lie in
 // different banks.
 constexpr int kExpandRows = kExpandWaves * kRows;
-constexpr int kThreads = kExpandWaves * kWave;
 template <bool GLU>
 __device__ __forceinline__ int block_col(int r) {      // block row -> its column of y (and half)
     return GLU ? (r & 31) : r;
@@ -326,11 +326,14 @@ __device__ __forceinline__ int lds_row(int r) {        // -> its place: tile by 
 // The wave's rows `mask` of one adapter (of none: slot -1) against columns
 // [first, last) of y: CC chunks of 32 ranks (HALF: max_rank 16, where an
 // instruction's 32 k hold the 16 ranks twice, under two pieces of z; CC 0:
-// base alone).  All waves of the work-group come here together, also those
-// without such rows (mask 0), which only bring B.
-template <bool GLU, int CC, bool HALF, bool BB>
+// base alone).  All NW waves of the work-group come here together, also those
+// without such rows (mask 0), which only bring B.  ZL: z of the wave's rows
+// lies in the LDS, in the workspace's order.
+template <bool GLU, int CC, bool HALF, bool BB, int NW, bool ZL>
 __device__ __forceinline__ void expand_cols(const LoraArgs& p, int splits, int slot, int rank, uint32_t mask,
-                                            int64_t row0, int first, int last, int width, u32x4* lds) {
+                                            int64_t row0, int first, int last, int width, u32x4* lds,
+                                            const f32x4* zl) {
+    constexpr int kThreads = NW * kWave;
     constexpr int W = GLU ? 2 : 4, NP = GLU ? 2 : 1, C = CC ? CC : 1;
     constexpr int PH = C < 2 ? C : 2;                 // chunks of one pass through the LDS
     constexpr int P = HALF ? 2 : PH * 4;              // pieces of a row in a pass
@@ -388,18 +391,24 @@ __device__ __forceinline__ void expand_cols(const LoraArgs& p, int splits, int s
 #pragma unroll
             for (int c = 0; c < C; ++c) {
                 const int r = HALF ? (q & 1) * 8 : c * 32 + q * 8;
-                const int64_t apart = z_run(p, 1, 0, 0, 0) - z_run(p, 0, 0, 0, 0);
-                const f32x4* z0 = z_run(p, 0, row0 / kRows, c, 0) + (HALF ? lane & 31 : lane);
+                const int at = HALF ? lane & 31 : lane;
                 f32x4 lo = {}, hi = {};
-                for (int s = 0; s < splits; s += 2) {
-                    const f32x4* z1 = z0 + s * apart;
-                    const f32x4* z2 = z0 + min(s + 1, splits - 1) * apart;
-                    const f32x4 l1 = z1[0], h1 = z1[kWave], l2 = z2[0], h2 = z2[kWave];
-                    lo += l1;
-                    hi += h1;
-                    if (s + 1 < splits) {
-                        lo += l2;
-                        hi += h2;
+                if constexpr (ZL) {
+                    lo = zl[c * 2 * kWave + at];
+                    hi = zl[(c * 2 + 1) * kWave + at];
+                } else {
+                    const int64_t apart = z_run(p, 1, 0, 0, 0) - z_run(p, 0, 0, 0, 0);
+                    const f32x4* z0 = z_run(p, 0, row0 / kRows, c, 0) + at;
+                    for (int s = 0; s < splits; s += 2) {
+                        const f32x4* z1 = z0 + s * apart;
+                        const f32x4* z2 = z0 + min(s + 1, splits - 1) * apart;
+                        const f32x4 l1 = z1[0], h1 = z1[kWave], l2 = z2[0], h2 = z2[kWave];
+                        lo += l1;
+                        hi += h1;
+                        if (s + 1 < splits) {
+                            lo += l2;
+                            hi += h2;
+                        }
                     }
                 }
                 float z[8];
@@ -496,7 +505,8 @@ __device__ __forceinline__ void expand_cols(const LoraArgs& p, int splits, int s
 // least nblocks.  How many adapters a tile names is known here only: one for
 // most tiles of a prompt, dozens for sequences decoding together.
 template <bool GLU, int MC, bool BB>
-__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(MC > 2 ? 2 : 4))) void lora_expand_kernel(
+__global__ __launch_bounds__(kExpandWaves* kWave)
+    __attribute__((amdgpu_waves_per_eu(MC > 2 ? 2 : 4))) void lora_expand_kernel(
     LoraArgs p, int splits, int share, int nblocks) {
     constexpr int kMaxPitch = (MC == 0 ? 2 : MC == 1 ? 4 : 8) + 1;
     __shared__ u32x4 lds[2 * 64 * kMaxPitch];
@@ -533,7 +543,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(MC > 2
         const uint32_t mask = uint32_t(__ballot(t.in && t.slot == slot) >> (wave * kRows)) & 0xFFFFu;
         const int rank = slot < 0 ? 0 : min(max(p.rank[slot], 0), p.R);
 #define GRIM_COLS(CC, HALF) \
-    expand_cols<GLU, CC, HALF, BB>(p, splits, slot, rank, mask, row0, first, last, width, lds)
+    expand_cols<GLU, CC, HALF, BB, kExpandWaves, false>(p, splits, slot, rank, mask, row0, first, last, width, lds, nullptr)
         if (rank == 0) {
             if (copy) GRIM_COLS(0, false);
         } else if constexpr (MC == 0) {
@@ -545,6 +555,88 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(MC > 2
             else GRIM_COLS(MC, false);
         }
 #undef GRIM_COLS
+    }
+}
+
+// --------------------------------------------------------- both in one launch
+
+// A few rows (one tile of 16) of small adapters: every work-group forms the z
+// that it needs itself, all of K over its eight waves, and goes on to its
+// columns.  What it costs is A once a work-group from the L2, what it saves
+// is a launch and the trip of z through memory.
+template <bool GLU, bool XB, bool BB, int NR>
+__global__ __launch_bounds__(kShrinkWaves* kWave) void lora_one_kernel(LoraArgs p, int share) {
+    constexpr int MC = NR == 1 ? 0 : NR == 2 ? 1 : 2;
+    constexpr int kMaxPitch = (MC == 0 ? 2 : MC == 1 ? 4 : 8) + 1, kRegion = NR * 16 * 8 + kRows * (XB ? 8 : 16);
+    // shrink's regions; then expand's two buffers
+    __shared__ u32x4 lds[kShrinkWaves][kRegion];
+    static_assert(kShrinkWaves * kRegion >= 2 * 64 * kMaxPitch, "expand's buffers lie in shrink's regions");
+    __shared__ f32x4 zl[(MC < 2 ? 1 : 2) * 2 * kWave];
+    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+    const int q = lane >> 4, col = lane & 15;
+    constexpr int kBlock = GLU ? 32 : 64;
+    const int width = GLU ? p.N / 2 : p.N;
+    const int blocks = (width + kBlock - 1) / kBlock, ksteps = (p.K + kStep - 1) / kStep;
+    const Tile t = tile_rows<kRows>(p, 0);
+    const bool copy = GLU || p.base != p.y;
+    uint64_t todo = (copy ? __ballot(t.in) : __ballot(t.slot >= 0)) & 0xFFFFu;
+    int count = 0, slots = 0;
+    while (todo) {
+        int lead;
+        const int slot = next_slot(t, todo, lead);
+        slots = lane == count ? slot : slots;
+        ++count;
+    }
+    const int total = count * blocks, run = (total + share - 1) / share;
+    int at = int(blockIdx.x) * run;
+    const int end = min(total, at + run);
+    while (at < end) {
+        const int g = at / blocks, b0 = at - g * blocks, n = min(end - at, blocks - b0);
+        at += n;
+        const int first = b0 * kBlock, last = min(width, first + n * kBlock);
+        const int slot = __builtin_amdgcn_readlane(slots, g);
+        const uint32_t mask = uint32_t(__ballot(t.in && t.slot == slot)) & 0xFFFFu;
+        const int rank = slot < 0 ? 0 : min(max(p.rank[slot], 0), p.R);
+        const int nr = min(NR, (rank + 15) / 16);
+        if (nr > 0) {
+            f32x4 acc[4] = {};
+            int ln = lane;                                  // opaque: see expand_cols
+            asm volatile("" : "+v"(ln));
+            const int lead = __builtin_ctz(mask);
+#define GRIM_STEPS(NF) shrink_steps<XB, NF>(p, slot, 0, mask, 0, lead, ln, wave, ksteps, lds[wave], acc)
+            if (NR == 1 || nr == 1) GRIM_STEPS(1);
+            else if (NR == 2 || nr == 2) GRIM_STEPS(2);
+            else GRIM_STEPS(4);
+#undef GRIM_STEPS
+#pragma unroll
+            for (int r = 0; r < NR; ++r)
+                if (r < nr) __builtin_memcpy(&lds[wave][r * kWave + lane], &acc[r], 16);
+            __syncthreads();
+            if (wave < nr) {
+                f32x4 z = {};
+#pragma unroll
+                for (int w = 0; w < kShrinkWaves; ++w) {
+                    f32x4 o;
+                    __builtin_memcpy(&o, &lds[w][wave * kWave + lane], 16);
+                    z += o;
+                }
+                zl[((wave >> 1) * 2 + (q & 1)) * kWave + ((wave & 1) * 2 + (q >> 1)) * 16 + col] = z;
+            }
+            __syncthreads();
+        }
+        const uint32_t mine = wave == 0 ? mask : 0;
+#define GRIM_COLS(CC, HALF) \
+    expand_cols<GLU, CC, HALF, BB, kShrinkWaves, true>(p, 1, slot, rank, mine, 0, first, last, width, lds[0], zl)
+        if (rank == 0) {
+            if (copy) GRIM_COLS(0, false);
+        } else if constexpr (MC == 0) {
+            GRIM_COLS(1, true);
+        } else {
+            if (MC == 1 || rank <= 32) GRIM_COLS(1, false);
+            else GRIM_COLS(MC, false);
+        }
+#undef GRIM_COLS
+        __syncthreads();                                    // the next z takes the buffers and zl
     }
 }
 
@@ -597,13 +689,44 @@ void expand(hipStream_t st, const LoraArgs& a, int splits) {
     if (share > most) share = most;
     const dim3 grid(unsigned(share) * tiles);
 #define GRIM_EXPAND(MC) \
-    hipLaunchKernelGGL((lora_expand_kernel<GLU, MC, BB>), grid, dim3(kThreads), 0, st, a, splits, int(share), nb)
+    hipLaunchKernelGGL((lora_expand_kernel<GLU, MC, BB>), grid, dim3(kExpandWaves * kWave), 0, st, a, splits, int(share), nb)
     if (a.R <= 16) GRIM_EXPAND(0);
     else if (a.R <= 32) GRIM_EXPAND(1);
     else if (a.R <= 64) GRIM_EXPAND(2);
     else if (a.R <= 128) GRIM_EXPAND(4);
     else GRIM_EXPAND(8);
 #undef GRIM_EXPAND
+}
+
+// One launch takes up to 16 rows where a wave has at most four steps of K and
+// a work-group (one a CU) at most two blocks of columns, every row an adapter
+// of its own.  As a graph, one launch against two: one row, 768 -> 2048, rank
+// 16: 5.2, 7.4 us; 2048 -> 2048: 7.3, 7.9 (rank 64: 10.1, 10.4); 4096 ->
+// 4096: 10.8, 8.8; 16 rows 2048 -> 2048: 8.1, 9.3; 2048 -> 7168: 11.3, 10.2.
+// Called one by one the launch saved counts 3 us more.
+constexpr int kOneSteps = 4, kOneGroups = 256, kOneBlocks = 2;
+int one_groups(const LoraArgs& a) {
+    if (a.T > kRows || a.R > 64 || a.K > kOneSteps * kShrinkWaves * kStep) return 0;
+    const int width = a.glu ? a.N / 2 : a.N, block = a.glu ? 32 : 64;
+    const int64_t work = int64_t(a.T) * ((width + block - 1) / block);
+    return work > kOneGroups * kOneBlocks ? 0 : int(work < kOneGroups ? work : kOneGroups);
+}
+
+template <bool GLU, bool XB>
+void one(hipStream_t st, const LoraArgs& a, int groups) {
+#define GRIM_ONE(BB, NR) \
+    hipLaunchKernelGGL((lora_one_kernel<GLU, XB, BB, NR>), dim3(groups), dim3(kShrinkWaves * kWave), 0, st, a, groups)
+#define GRIM_ONE_R(BB)               \
+    if (a.R <= 16) GRIM_ONE(BB, 1);  \
+    else if (a.R <= 32) GRIM_ONE(BB, 2); \
+    else GRIM_ONE(BB, 4)
+    if (a.base_bf16) {
+        GRIM_ONE_R(true);
+    } else {
+        GRIM_ONE_R(false);
+    }
+#undef GRIM_ONE_R
+#undef GRIM_ONE
 }
 
 }  // namespace
@@ -618,6 +741,11 @@ size_t lora_workspace_bytes(int K, int R, int T) {
 
 hipError_t lora_launch(hipStream_t st, const LoraArgs& a) {
     if (a.T <= 0) return hipSuccess;
+    if (const int groups = one_groups(a)) {
+        if (a.glu) a.x_bf16 ? one<true, true>(st, a, groups) : one<true, false>(st, a, groups);
+        else a.x_bf16 ? one<false, true>(st, a, groups) : one<false, false>(st, a, groups);
+        return hipGetLastError();
+    }
     const int splits = lora_splits(a.K, a.T);
     // distinct adapters a tile can name, rows without one among them
     const int items = a.T > kItemRows ? 1 : a.T < kRows ? a.T : kRows;

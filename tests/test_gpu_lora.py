@@ -174,6 +174,18 @@ def test_a_row_does_not_depend_on_the_others(gpu, T, order):
     assert torch.equal(y[d["slot"] != 2], z[d["slot"] != 2])
 
 
+@pytest.mark.parametrize("T,K,N", [(1, 2048, 264), (1, 2056, 264), (7, 520, 2056), (16, 2048, 2048), (16, 64, 2056),
+                                   (17, 64, 64)])
+@pytest.mark.parametrize("R", [16, 32, 48, 64, 80])
+def test_one_launch_and_two(gpu, T, K, N, R):
+    """Around the sizes up to which a few rows take one launch."""
+    for order, x_bf16, y_bf16 in (("mixed", False, False), ("mixed", True, True), ("runs", False, True)):
+        d = make(T, K, N, 5, R, T + K + R, order, x_bf16, y_bf16)
+        check(d, gpu, y_bf16=y_bf16)
+        check(d, gpu, inplace=True)
+        check(d, gpu, glu=True, y_bf16=not y_bf16)
+
+
 def test_full_ranks_and_many_adapters_in_a_tile(gpu):
     """64 adapters in the 64 rows of a tile, each rank of the storage."""
     for R in (16, 32, 48, 64, 80, 128, 256):
