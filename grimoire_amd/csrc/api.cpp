@@ -292,6 +292,27 @@ int grimoire_moe_router_topk_group(void* stream, const float* logits, const floa
     return topk_common(stream, a);
 }
 
+// Rows of an argument in memory: bytes from row to row and of a row.
+struct RowSpan {
+    const void* p;
+    int64_t stride, width, rows;
+};
+
+// Whether two arguments share memory.  Rows at one distance may lie beside
+// each other in one buffer (column slices); at different distances their
+// whole ranges must be apart.
+static bool share_memory(const RowSpan& a, const RowSpan& b) {
+    if (!a.p || !b.p || a.rows <= 0 || b.rows <= 0) return false;
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a.p), y = reinterpret_cast<uintptr_t>(b.p);
+    if (x + (a.rows - 1) * a.stride + a.width <= y || y + (b.rows - 1) * b.stride + b.width <= x) return false;
+    if (a.stride != b.stride || a.rows == 1 || b.rows == 1) return true;
+    const int64_t d = x <= y ? int64_t(y - x) % a.stride : (a.stride - int64_t(x - y) % a.stride) % a.stride;
+    return d < a.width || d + b.width > a.stride;
+}
+static bool same_rows(const RowSpan& a, const RowSpan& b) {
+    return a.p == b.p && a.stride == b.stride && a.width == b.width;
+}
+
 int grimoire_moe_router_scores(void* stream, const grim_score_params* p, const void* logits,
                                int logits_bf16, int64_t row_stride, int tokens, int n_experts,
                                int top_k, int32_t* out_expert, float* out_weight) {
@@ -315,6 +336,11 @@ int grimoire_moe_router_scores(void* stream, const grim_score_params* p, const v
         if (top_k > p->topk_group * (n_experts / G))
             return fail(GRIM_ERR_SHAPE, "top_k exceeds the experts of the kept groups");
     }
+    const int64_t size = logits_bf16 ? 2 : 4, picks = int64_t(top_k) * 4;
+    const RowSpan in{logits, row_stride * size, n_experts * size, tokens};
+    const RowSpan ids{out_expert, picks, picks, tokens}, weights{out_weight, picks, picks, tokens};
+    if (share_memory(in, ids) || share_memory(in, weights) || share_memory(ids, weights))
+        return fail(GRIM_ERR_ARG, "logits and outputs overlap");
     ScoresArgs a{logits, row_stride, logits_bf16 ? 1 : 0, tokens, n_experts, top_k,
                  p->score == GRIM_SCORE_SIGMOID, p->bias, G, G > 1 ? p->topk_group : 1,
                  p->group_score == GRIM_GROUP_TOP2, p->normalize, p->scaling, out_expert, out_weight};
@@ -473,6 +499,26 @@ int grimoire_rmsnorm_residual(void* stream, float* h, const float* r0, const flo
     return status(combine_norm_launch(S(stream), a));
 }
 
+// An output of a block norm may take the place of an input of its own layout
+// (each row is read before it is written) and overlaps nothing else.
+static bool norm_overlap(const BlockNormArgs& a, std::initializer_list<RowSpan> inputs) {
+    const int64_t f = int64_t(a.H) * 4, b = int64_t(a.H) * 2;
+    const RowSpan outs[3] = {{a.h_out, f, f, a.T}, {a.out, f, f, a.T}, {a.out_bf, b, b, a.T}};
+    for (int i = 0; i < 3; ++i) {
+        for (const RowSpan& in : inputs)
+            if (share_memory(outs[i], in) && !same_rows(outs[i], in)) return true;
+        for (int j = 0; j < i; ++j)
+            if (share_memory(outs[i], outs[j])) return true;
+    }
+    return false;
+}
+static RowSpan gate_span(const BlockNormArgs& a) {
+    const int64_t size = a.gate_bf16 ? 2 : 4;
+    if (a.gate_kind == GRIM_GATE_FULL) return {a.gate, a.H * size, a.H * size, a.T};
+    const int64_t n = (a.gate_kind == GRIM_GATE_ROW ? a.T : a.H) * size;
+    return {a.gate, n, n, 1};
+}
+
 static bool aligned(const void* p, uintptr_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 
 // What both forms of the block norm check and share.
@@ -512,6 +558,9 @@ int grimoire_block_norm(void* stream, const grim_block_norm_params* p, const voi
         return fail(GRIM_ERR_SHAPE, "x_stride=%lld (need >= hidden, %% 4)", (long long)x_stride);
     if (!aligned(x, x_bf16 ? 8 : 16)) return fail(GRIM_ERR_ARG, "x alignment");
     a.x = x; a.x_bf16 = x_bf16 ? 1 : 0; a.x_stride = x_stride;
+    const int64_t size = x_bf16 ? 2 : 4, row = int64_t(hidden) * 4;
+    if (norm_overlap(a, {{h, row, row, tokens}, {x, x_stride * size, hidden * size, tokens}, gate_span(a)}))
+        return fail(GRIM_ERR_ARG, "an output overlaps another argument");
     return status(block_norm_launch(S(stream), a));
 }
 
@@ -527,6 +576,10 @@ int grimoire_moe_block_norm(void* stream, const grim_block_norm_params* p, const
     if (routed_rows < 0) return fail(GRIM_ERR_SHAPE, "routed_rows=%d", routed_rows);
     if (!aligned(routed, 8) || !aligned(shared, 16)) return fail(GRIM_ERR_ARG, "routed/shared alignment");
     a.routed = routed; a.routed_rows = routed_rows; a.inverse = inverse; a.rw = route_weight; a.shared = shared; a.K = top_k;
+    const int64_t row = int64_t(hidden) * 4, all = int64_t(routed_rows) * hidden * 2, picks = int64_t(tokens) * top_k * 4;
+    if (norm_overlap(a, {{h, row, row, tokens}, {shared, row, row, tokens}, gate_span(a), {routed, all, all, routed_rows ? 1 : 0},
+                         {inverse, picks, picks, 1}, {route_weight, picks, picks, 1}}))
+        return fail(GRIM_ERR_ARG, "an output overlaps another argument");
     return status(block_norm_launch(S(stream), a));
 }
 
@@ -560,6 +613,11 @@ static int lora_common(void* stream, const grim_lora* L, const int32_t* row_slot
         return fail(GRIM_ERR_ARG, "adapters, x and fp32 rows 16-byte, bf16 rows 8-byte alignment");
     if (y == base && (glu || !base_bf16 != !y_bf16 || base_stride != y_stride))
         return fail(GRIM_ERR_ARG, "in place needs the same type and stride (and no SwiGLU)");
+    const int64_t xz = x_bf16 ? 2 : 4, bz = base_bf16 ? 2 : 4, yz = y_bf16 ? 2 : 4;
+    const RowSpan out{y, y_stride * yz, width * yz, rows};
+    if (share_memory(out, {x, x_stride * xz, L->K * xz, rows}) ||
+        (y != base && share_memory(out, {base, base_stride * bz, L->N * bz, rows})))
+        return fail(GRIM_ERR_ARG, "the output overlaps x or base");
     const size_t need = lora_workspace_bytes(L->K, L->max_rank, rows);
     if (!ws || ws_bytes < need) return fail(GRIM_ERR_WORKSPACE, "adapter workspace too small (need %zu)", need);
     if (!aligned(ws, 16)) return fail(GRIM_ERR_ARG, "workspace not 16-byte aligned");

@@ -14,7 +14,7 @@
 //
 // Where it stands (us, shrink + expand, and what their bytes take at the 4.94
 // TB/s of a large copy): 4096 rows of 9 requests, 2048 -> 7168, rank 64 of
-// mixed ranks, bf16: 13 + 35 (28; base copied to y by the same loop 25.5);
+// mixed ranks, bf16: 13 + 37 (28; base copied to y by the same loop 25.5);
 // 2001 rows of 5, 2880 -> 2 x 2880, rank 16, fp32: 11 + 19 (19); 48 mixed
 // rows of 32 adapters, 2048 -> 7168: 6 + 12 (3.3); one row, 768 -> 2048: 5 in
 // one launch, a chain of dependent loads.

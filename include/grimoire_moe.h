@@ -181,7 +181,7 @@ int grimoire_moe_router_topk_group(void* stream, const float* logits, const floa
  * expert -1, weight 0 (the products skip such routes).  Scores, sums and the
  * choice are fp64, so the routing does not depend on fp32 rounding.
  * logits: fp32 or (logits_bf16) bf16 rows, row_stride elements apart
- * (>= n_experts).  n_experts <= 512, top_k <= min(16, n_experts), and with
+ * (>= n_experts), apart from both outputs.  n_experts <= 512, top_k <= min(16, n_experts), and with
  * groups <= topk_group * (n_experts / n_group). */
 enum grim_score {
     GRIM_SCORE_SOFTMAX = 0,
@@ -368,7 +368,8 @@ int grimoire_rmsnorm_residual(void* stream, float* h, const float* r0, const flo
  * h_out = h' (may be NULL, may be h), out = o in fp32, out_bf = o in bf16
  * (either may be NULL; without both, pre_weight may be NULL).  The norm
  * weights are bf16 [hidden].  hidden % 4 == 0, <= 32768; fp32 rows 16-byte,
- * bf16 rows 8-byte aligned.
+ * bf16 rows 8-byte aligned.  An output may take the place of an input of its
+ * own type and row distance; it overlaps nothing else.
  *   grimoire_block_norm: f = x[t], fp32 or (x_bf16) bf16 rows x_stride
  *     elements apart (a multiple of 4, >= hidden).
  *   grimoire_moe_block_norm: f = shared[t] (fp32, may be NULL) + sum_s
@@ -428,10 +429,13 @@ size_t grimoire_lora_workspace_bytes(const grim_lora* L, int rows);
 /* y[t] = base[t] + scale_a B_a (A_a x[t]); rows without an adapter are
  * copied (in place: left as they are).  x [rows][K], base and y [rows][N]:
  * fp32 or bf16 rows, *_stride elements apart (x a multiple of 8, base and y
- * of 4; at most 2^24), max_rank * K and max_rank * N at most 2^29; fp32 and x rows 16-byte, bf16 base and y rows 8-byte aligned.  y may
- * be base (same type and stride) and overlaps nothing else.  Sums are fp32,
- * in an order that does not depend on the other rows' adapters; fp32
- * activations are multiplied in full precision. */
+ * of 4; at most 2^24), max_rank * K and max_rank * N at most 2^29; fp32 and x
+ * rows 16-byte, bf16 base and y rows 8-byte aligned.  y may be base (same
+ * type and stride) and overlaps nothing else; rows at one distance may lie
+ * beside each other in one buffer.  Sums are fp32, in an order that does not
+ * depend on the other rows' adapters; fp32 activations are multiplied in full
+ * precision.  An adapter weight that is not finite makes NaN or infinity of
+ * what it is multiplied into, in its own adapter's rows only. */
 int grimoire_lora_add(void* stream, const grim_lora* L, const int32_t* row_slot, const void* x, int x_bf16,
                       int64_t x_stride, const void* base, int base_bf16, int64_t base_stride, void* y,
                       int y_bf16, int64_t y_stride, int rows, void* workspace, size_t workspace_bytes);

@@ -137,3 +137,45 @@ def test_cpu_tensors_and_bad_names():
         ops.BlockNorm(None)(torch.zeros(2, 8), torch.zeros(2, 8), torch.zeros(2, 8))
     with pytest.raises(_abi.GrimoireError):
         ops.BlockNorm(None, gate="head")
+
+
+M = 1 << 20   # arguments that lie apart
+
+
+@pytest.mark.parametrize("kw", [
+    dict(ids=M, w=2 * M, logits=M), dict(ids=M, w=2 * M, logits=2 * M + 60), dict(ids=M, w=M + 60, logits=4 * M),
+    dict(ids=M, w=2 * M, logits=M - 256)])
+def test_scores_overlap(kw):
+    assert scores(**kw) == ARG
+
+
+@pytest.mark.parametrize("kw", [
+    dict(h_out=M + 16), dict(out=M + 256), dict(out=2 * M - 16), dict(out_bf=2 * M), dict(out=3 * M),
+    dict(out_bf=3 * M + 256), dict(x=3 * M + 256, x_stride=128), dict(x=3 * M + 256, x_stride=128, x_bf16=1),
+    dict(x=3 * M, x_stride=128), dict(gate_kind=3, gate=3 * M, gate_bf16=1), dict(gate_kind=2, gate=3 * M + 16),
+    dict(gate_kind=1, gate=4 * M + 256)])
+def test_block_norm_overlap(kw):
+    args = dict(h=M, x=2 * M, h_out=3 * M, out=4 * M, out_bf=None)
+    args.update(kw)
+    assert norm(**args) == ARG
+
+
+@pytest.mark.parametrize("kw", [dict(routed=4 * M + 496), dict(inverse=4 * M + 508), dict(rw=4 * M), dict(rw=5 * M + 8),
+                                dict(shared=4 * M + 256), dict(h=5 * M - 256)])
+def test_moe_block_norm_overlap(kw):
+    p = _abi.BlockNormParams(pre_weight=A, eps=1e-6)
+    a = dict(h=M, routed=2 * M, inverse=3 * M, rw=3 * M + 64, shared=None)
+    a.update(kw)
+    assert _abi.lib().grimoire_moe_block_norm(None, C.byref(p), None, 0, a["h"], a["routed"], 9, a["inverse"], a["rw"],
+                                              a["shared"], 4 * M, None, 5 * M, 2, 4, 64) == ARG
+
+
+@pytest.mark.parametrize("kw", [
+    dict(y=M), dict(y=M + 256), dict(y=M - 64), dict(y=2 * M + 64), dict(y=2 * M, base_stride=64, y_stride=36),
+    dict(glu=True, y=2 * M + 64), dict(y=2 * M + 112, base_stride=64, y_stride=64),
+    dict(y=M + 128, x_stride=96, y_stride=96), dict(y=M + 240, x_stride=96, y_stride=96),
+    dict(y=M, y_bf16=1, x_bf16=1), dict(y=2 * M, y_bf16=1)])
+def test_lora_overlap(kw):
+    args = dict(x=M, base=2 * M, y=3 * M)
+    args.update(kw)
+    assert lora(**args) == ARG
