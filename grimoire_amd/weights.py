@@ -249,8 +249,13 @@ class LoraAdapters:
 
     def load(self, slot: int, a: torch.Tensor, b: torch.Tensor, scale: float) -> None:
         """An adapter's A [r][K] and B [N][r] into a slot (r <= max_rank;
-        rounded to bf16 when they are not), in the current stream's order."""
-        r = a.shape[0]
+        rounded to bf16 when they are not; int16: bf16 bits), in the current
+        stream's order."""
+        r = a.shape[0] if a.dim() == 2 else -1
+        # bf16 as int16 bits, as in the slots themselves
+        a, b = (t.view(torch.bfloat16) if t.dtype == torch.int16 else t for t in (a, b))
+        if not (a.is_floating_point() and b.is_floating_point()):
+            raise _abi.GrimoireError(f"adapter: {a.dtype} and {b.dtype}, expected floating point or bf16 bits")
         if not 0 <= slot < self.slots or r > self.max_rank or a.shape != (r, self.K) or b.shape != (self.N, r):
             raise _abi.GrimoireError(f"slot {slot}: A {tuple(a.shape)}, B {tuple(b.shape)} for "
                                      f"[{self.N}][{self.K}] of rank <= {self.max_rank}")

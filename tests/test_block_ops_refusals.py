@@ -179,3 +179,17 @@ def test_lora_overlap(kw):
     args = dict(x=M, base=2 * M, y=3 * M)
     args.update(kw)
     assert lora(**args) == ARG
+
+
+def test_lora_adapters_load_bits():
+    """bf16 bits held as int16 are loaded as what they stand for."""
+    ad = weights.LoraAdapters.empty(2, 16, 64, 32, device="cpu")
+    a, b = torch.randn(3, 64).bfloat16(), torch.randn(32, 3).bfloat16()
+    ad.load(1, a.view(torch.int16), b.view(torch.int16), 1.0)
+    assert torch.equal(ad.a[1, :3], a) and torch.equal(ad.b[1, :, :3], b)
+    bits = weights.LoraAdapters(ad.a.view(torch.int16), ad.b.view(torch.int16), ad.rank, ad.scale)
+    bits.load(0, a.float(), b, 1.0)
+    assert torch.equal(ad.a[0, :3], a) and torch.equal(ad.b[0, :, :3], b)
+    for bad in (torch.ones(3, 64, dtype=torch.int32), torch.ones(64), torch.ones(3, 64, dtype=torch.int8)):
+        with pytest.raises(_abi.GrimoireError):
+            ad.load(0, bad, b, 1.0)
