@@ -372,12 +372,15 @@ class RouteScores:
         if bias is not None:
             _dev(bias)
             _flat(bias, "bias", (bias.numel(),), _F32, bias.get_device())
-        self.bias = bias
+        self._bias = bias
         self.struct = _abi.ScoreParams(self.SCORES[score], n_group, topk_group, self.GROUPS[group_score],
                                        int(normalize), float(scaling), _p(bias))
         self._bias_of = None if bias is None else (bias.numel(), bias.get_device())
         self._call = lib().grimoire_moe_router_scores
         self._ref = C.byref(self.struct)
+
+    # what the struct points at: kept as long as it is, never another
+    bias = property(lambda self: self._bias)
 
     def __call__(self, logits, out_expert, out_weight, stream=None):
         """Routes of logits [T][E] (fp32 or bf16, rows may lie apart) into
@@ -410,7 +413,7 @@ class BlockNorm:
             if w is not None:
                 _dev(w)
                 _flat(w, "norm weight", (w.numel(),), _B16, w.get_device())
-        self.pre_weight, self.post_weight, self.gate = pre_weight, post_weight, gate
+        self._pre, self._post, self._gate = pre_weight, post_weight, gate
         self._weights_of = {(w.numel(), w.get_device()) for w in (pre_weight, post_weight) if w is not None}
         self._dense, self._moe = lib().grimoire_block_norm, lib().grimoire_moe_block_norm
         self.struct = _abi.BlockNormParams(_p(post_weight), _p(pre_weight), float(weight_offset), float(eps),
@@ -418,13 +421,18 @@ class BlockNorm:
                                            int(gate_sigmoid))
         self._ref = C.byref(self.struct)
 
+    # what the struct points at and was made for: never another
+    pre_weight = property(lambda self: self._pre)
+    post_weight = property(lambda self: self._post)
+    gate = property(lambda self: self._gate)
+
     def _args(self, h, h_out, out, out_bf, gate):
         dev = _gpu(h)
         T, H = shape = h.shape
         for of in self._weights_of:
             if of != (H, dev):
                 raise _abi.GrimoireError("norm weights: one value a column, on h's device")
-        kind = self.gate
+        kind = self._gate
         if (gate is not None) != (kind != "none"):
             raise _abi.GrimoireError(f"gate {kind!r} and the gate tensor do not go together")
         gp, g16 = None, 0
@@ -461,12 +469,14 @@ class BlockNorm:
 class Lora:
     """Low-rank adapters of many requests beside one shared projection
     (grimoire_lora_add / grimoire_lora_swiglu), with the workspace of up to
-    max_rows rows: calls of one object must not overlap.  What changes in the
-    adapters' tensors (`LoraAdapters.load`) holds for the next call."""
+    max_rows rows: calls of one object must not overlap, and the object stays
+    while a graph or a stream other than the one it was made on has calls of it
+    to run.  What changes in the adapters' tensors (`LoraAdapters.load`) holds
+    for the next call."""
 
     def __init__(self, adapters: LoraAdapters, max_rows: int):
         _dev(adapters.a)
-        self.adapters = adapters
+        self._adapters, self._KN = adapters, (adapters.K, adapters.N)
         self.struct = adapters.struct()
         self.max_rows = max_rows
         self.dev = adapters.a.get_device()
@@ -475,16 +485,18 @@ class Lora:
         self._ref = C.byref(self.struct)
         self._add, self._swiglu = lib().grimoire_lora_add, lib().grimoire_lora_swiglu
 
+    adapters = property(lambda self: self._adapters)
+
     def _call(self, fn, what, row_slot, x, base, y, width, stream):
         _gpu(x)
-        A, dev = self.adapters, self.dev
+        (K, N), dev = self._KN, self.dev
         T = x.shape[0]
         if T > self.max_rows:
             raise _abi.GrimoireError("more rows than the workspace was sized for")
         if x.get_device() != dev or base.get_device() != dev or y.get_device() != dev:
             raise _abi.GrimoireError(f"{what}: x, base, output and adapters on different devices")
-        xp, x16, xs = _rows(x, "x", A.K, T)
-        bp, b16, bs = _rows(base, "base", A.N, T)
+        xp, x16, xs = _rows(x, "x", K, T)
+        bp, b16, bs = _rows(base, "base", N, T)
         yp, y16, ys = _rows(y, "output", width, T)
         _launch(dev, stream, fn, what, self._ref, _flat(row_slot, "row_slot", (T,), _I32, dev), xp, x16, xs, bp, b16,
                 bs, yp, y16, ys, T, self.workspace.data_ptr(), self.workspace.numel())
@@ -493,13 +505,12 @@ class Lora:
         """y = base + the adapters' product of x (base None: y += it).
         row_slot int32 [T]; x [T][K], base and y [T][N] fp32 or bf16, rows
         may lie apart."""
-        self._call(self._add, "lora_add", row_slot, x, y if base is None else base, y, self.adapters.N,
-                   stream)
+        self._call(self._add, "lora_add", row_slot, x, y if base is None else base, y, self._KN[1], stream)
 
     def swiglu(self, row_slot, x, base, h, stream=None):
         """h [T][N/2] = silu(gate) * up of the gate|up projection base
         [T][N] plus the adapters' product of x."""
-        self._call(self._swiglu, "lora_swiglu", row_slot, x, base, h, self.adapters.N // 2, stream)
+        self._call(self._swiglu, "lora_swiglu", row_slot, x, base, h, self._KN[1] // 2, stream)
 
 
 # ------------------------------------------------------------------- layer

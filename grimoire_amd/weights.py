@@ -217,18 +217,22 @@ class MoeLayer:
         return float(self.shared_gate_up.nbytes() + self.shared_down.nbytes())
 
 
-@dataclass
+@dataclass(frozen=True, eq=False)
 class LoraAdapters:
     """The low-rank adapters of one projection [N][K], in slots
     (grim_lora): a [slots][max_rank][K] and b [slots][N][max_rank] bf16 (or
     their bits as int16), rank int32 [slots], scale fp32 [slots], all on one
-    device.  What a slot holds past its rank is not part of its adapter."""
+    device.  What a slot holds past its rank is not part of its adapter.
+    The tensors are its for good: adapters come and go in their slots."""
     a: torch.Tensor
     b: torch.Tensor
     rank: torch.Tensor
     scale: torch.Tensor
 
     def __post_init__(self):
+        if self.a.dim() != 3 or self.b.dim() != 3:
+            raise _abi.GrimoireError(f"adapters: a {tuple(self.a.shape)}, b {tuple(self.b.shape)}, expected "
+                                     "[slots][max_rank][K] and [slots][N][max_rank]")
         S, R, K = self.a.shape
         N = self.b.shape[1]
         for t, shape, types in ((self.a, (S, R, K), (torch.bfloat16, torch.int16)),
@@ -237,7 +241,22 @@ class LoraAdapters:
             if t.shape != shape or t.dtype not in types or not t.is_contiguous() or t.device != self.a.device:
                 raise _abi.GrimoireError(f"adapters: {t.dtype} {tuple(t.shape)} on {t.device}, expected "
                                          f"contiguous {shape} on {self.a.device}")
-        self.slots, self.max_rank, self.K, self.N = S, R, K, N
+
+    @property
+    def slots(self) -> int:
+        return self.a.shape[0]
+
+    @property
+    def max_rank(self) -> int:
+        return self.a.shape[1]
+
+    @property
+    def K(self) -> int:
+        return self.a.shape[2]
+
+    @property
+    def N(self) -> int:
+        return self.b.shape[1]
 
     @staticmethod
     def empty(slots: int, max_rank: int, K: int, N: int, device="cuda") -> "LoraAdapters":

@@ -193,3 +193,18 @@ def test_lora_adapters_load_bits():
     for bad in (torch.ones(3, 64, dtype=torch.int32), torch.ones(64), torch.ones(3, 64, dtype=torch.int8)):
         with pytest.raises(_abi.GrimoireError):
             ad.load(0, bad, b, 1.0)
+
+
+def test_what_an_operator_was_made_for_stays():
+    """The structs hold addresses: the tensors behind them are not swapped."""
+    ad = weights.LoraAdapters.empty(2, 16, 64, 32, device="cpu")
+    assert (ad.slots, ad.max_rank, ad.K, ad.N) == (2, 16, 64, 32)
+    for obj, names in ((ad, ("a", "b", "rank", "scale", "K", "N", "slots", "max_rank")), (ops.RouteScores(), ("bias",)),
+                       (ops.BlockNorm(None), ("pre_weight", "post_weight", "gate"))):
+        for n in names:
+            with pytest.raises(AttributeError):
+                setattr(obj, n, getattr(obj, n))
+    with pytest.raises(_abi.GrimoireError):
+        weights.LoraAdapters(ad.a[0], ad.b, ad.rank, ad.scale)
+    with pytest.raises(_abi.GrimoireError):
+        weights.LoraAdapters(ad.a, ad.b[0], ad.rank, ad.scale)
