@@ -320,7 +320,7 @@ def _rows(t: torch.Tensor, what: str, width: int, rows: int):
     d = t.dtype
     if d is not _f32 and d is not _b16 and d is not _i16:
         raise _abi.GrimoireError(f"{what}: {d}, expected float32 or bfloat16")
-    return t.data_ptr(), d is not _f32, apart if rows > 1 or apart > width else width
+    return t.data_ptr(), d is not _f32, apart if rows > 1 else width   # one row: no distance
 
 
 def _flat(t: Optional[torch.Tensor], what: str, shape, dtypes, dev: int):
@@ -344,7 +344,12 @@ def _gpu(t: torch.Tensor) -> int:
 def _launch(dev: int, stream, fn, what: str, *args):
     """Call entry point fn(stream, *args) with device dev current and check
     its status; stream None: dev's current stream."""
-    s = _stream_now(dev) if stream is None else stream.cuda_stream
+    if stream is None:
+        s = _stream_now(dev)
+    elif stream.device_index != dev:
+        raise _abi.GrimoireError(f"{what}: a stream of another device than the tensors")
+    else:
+        s = stream.cuda_stream
     if _device_now() == dev:
         r = fn(s, *args)
     else:
@@ -428,6 +433,8 @@ class BlockNorm:
 
     def _args(self, h, h_out, out, out_bf, gate):
         dev = _gpu(h)
+        if h.dim() != 2:
+            raise _abi.GrimoireError("h: [T][H]")
         T, H = shape = h.shape
         for of in self._weights_of:
             if of != (H, dev):
@@ -452,14 +459,15 @@ class BlockNorm:
 
     def moe(self, h, routed, inverse, route_weight, shared, h_out, out=None, out_bf=None, gate=None, stream=None):
         """Behind routed experts (grimoire_moe_block_norm): routed bf16
-        [R][H] in dispatch order, inverse [T*K], route_weight [T][K]."""
+        [R][H] in dispatch order, inverse [T*K] or [T][K], route_weight
+        [T][K]."""
         T, H, dev, gp, g16, hp, hop, op, obp = self._args(h, h_out, out, out_bf, gate)
-        if route_weight.dim() != 2:
-            raise _abi.GrimoireError("route_weight: [T][K]")
+        if route_weight.dim() != 2 or routed.dim() != 2:
+            raise _abi.GrimoireError("routed [R][H], route_weight [T][K]")
         K = route_weight.shape[1]
         _launch(dev, stream, self._moe, "moe_block_norm", self._ref, gp, g16, hp,
                 _flat(routed, "routed", (routed.shape[0], H), _B16, dev), routed.shape[0],
-                _flat(inverse.view(-1), "inverse", (T * K,), _I32, dev),
+                _flat(inverse, "inverse", (T * K,) if inverse.dim() == 1 else (T, K), _I32, dev),
                 _flat(route_weight, "route_weight", (T, K), _F32, dev), _flat(shared, "shared", (T, H), _F32, dev), hop,
                 op, obp, T, K, H)
 
@@ -490,6 +498,8 @@ class Lora:
     def _call(self, fn, what, row_slot, x, base, y, width, stream):
         _gpu(x)
         (K, N), dev = self._KN, self.dev
+        if x.dim() != 2:
+            raise _abi.GrimoireError("x: [T][K]")
         T = x.shape[0]
         if T > self.max_rows:
             raise _abi.GrimoireError("more rows than the workspace was sized for")

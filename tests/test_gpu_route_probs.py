@@ -98,3 +98,45 @@ def test_refusals(gpu):
     bad = _abi.RouteParams(mode=4, scaling=1.0)
     with pytest.raises(_abi.GrimoireError):
         ops.MoeForward(fwd.L, cfg.T, bad, 0)(x, y)
+
+
+@pytest.mark.parametrize("c", CASES, ids=[c[1] for c in CASES])
+def test_too_few_experts_left(gpu, c):
+    """The bias takes experts out of service until fewer than K are left: the
+    free slots hold expert -1 and weight 0, and add nothing in any regime."""
+    print(f"probs, few left {c}", flush=True)
+    cfg, wl = layer((*c[:8], 1, 1, c[10]), gpu)
+    T, E, K = cfg.T, cfg.E, cfg.K
+    bias = torch.full((E,), float("-inf"))
+    left = torch.randperm(E, generator=torch.Generator().manual_seed(E))[:K - 1]
+    bias[left] = 0.0
+    Lg, dbias = wl.layer.to(gpu), bias.to(gpu)
+    fwd = ops.MoeForward(Lg, T, configs.route_params(cfg, dbias), c[0])
+    y = torch.full((T, cfg.H), float("nan"), device=gpu)
+    oe = torch.full((T, K), -7, dtype=torch.int32, device=gpu)
+    ow = torch.full((T, K), float("nan"), device=gpu)
+    fwd(wl.x.to(gpu), y, oe, ow)
+    torch.cuda.synchronize()
+    oe, ow = oe.cpu(), ow.cpu()
+    assert (oe[:, -1] == -1).all() and (ow[:, -1] == 0).all()
+    assert torch.equal(oe[:, :-1].sort(1).values, left.int().sort().values.expand(T, K - 1))
+    ids, w = oe.clone(), ow
+    ids[:, -1] = int(left[0])                    # the oracle's stand-in, of weight 0
+    assert_close(y.cpu(), O.moe_forward(wl.layer.struct(), ids, w, None, wl.x), what=cfg.name)
+
+
+def test_without_a_workspace(gpu):
+    """The library's own scratch serves this mode as the caller's does."""
+    for regime, T in ((0, 3), (1, 2), (7, 1), (2, 40)):
+        cfg, wl = layer((regime, "noalloc", T, 32, 4, 512, 256, "int8", 4, 2, False), gpu)
+        bias = wl.route_bias.to(gpu)
+        rp = configs.route_params(cfg, bias)
+        Lg, x = wl.layer.to(gpu), wl.x.to(gpu)
+        y0, y1 = torch.empty(T, cfg.H, device=gpu), torch.full((T, cfg.H), float("nan"), device=gpu)
+        fwd = ops.MoeForward(Lg, T, rp, regime)
+        fwd(x, y0)
+        r = _abi.lib().grimoire_moe_forward_noalloc(None, C.byref(fwd.struct), C.byref(rp), None, x.data_ptr(),
+                                                    y1.data_ptr(), T, None, None, regime)
+        assert r == 0, _abi.lib().grimoire_moe_last_error().decode()
+        torch.cuda.synchronize()
+        assert torch.equal(y0, y1)
