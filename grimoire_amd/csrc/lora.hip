@@ -16,7 +16,7 @@
 // TB/s of a large copy): 4096 rows of 9 requests, 2048 -> 7168, rank 64 of
 // mixed ranks, bf16: 13 + 37 (28; base copied to y by the same loop 25.5);
 // 2001 rows of 5, 2880 -> 2 x 2880, rank 16, fp32: 11 + 19 (19); 48 mixed
-// rows of 32 adapters, 2048 -> 7168: 6 + 12 (3.3); one row, 768 -> 2048: 5 in
+// rows of 32 adapters, 2048 -> 7168: 5 + 11 (3.3); one row, 768 -> 2048: 5 in
 // one launch, a chain of dependent loads.
 //
 // fp32 values are multiplied exactly: an fp32 x (and z) is the sum of three
@@ -89,13 +89,71 @@ __device__ __forceinline__ Tile tile_rows(const LoraArgs& p, int tile) {
     return t;
 }
 
-// The next distinct adapter among the rows `todo` (a bit a row), its first
-// row's lane in lead; takes its rows out of todo.
+// Where this lane's row stands among the distinct adapters that the rows `of`
+// name (no adapter counts as one more), in the order of their first rows.
+// Equal slots are found by a ballot a bit of their numbers, so that 64
+// adapters cost what two do (48 mixed rows of 32 adapters, 2048 -> 7168: 15.7
+// us; counted one after the other 17.7).
+struct Place {
+    uint64_t rows;   // the rows of its adapter, a bit each
+    bool first;      // it is the first of them
+    int index;       // first: its adapter's place
+    int count;       // of distinct adapters
+};
+
+__device__ __forceinline__ Place tile_places(const LoraArgs& p, const Tile& t, uint64_t of) {
+    const int lane = threadIdx.x & (kWave - 1);
+    Place w;
+    w.rows = of;
+    const uint32_t s = uint32_t(t.slot + 1);
+    for (uint32_t bit = 1; bit <= uint32_t(p.slots); bit <<= 1) {   // slots < 2^31: ends at 2^31
+        const uint64_t set = __ballot((s & bit) != 0);
+        w.rows &= (s & bit) ? set : ~set;
+    }
+    w.first = ((of >> lane) & 1) && (w.rows & ((uint64_t(1) << lane) - 1)) == 0;
+    const uint64_t firsts = __ballot(w.first);
+    w.index = __builtin_amdgcn_mbcnt_hi(uint32_t(firsts >> 32), __builtin_amdgcn_mbcnt_lo(uint32_t(firsts), 0));
+    w.count = __popcll(firsts);
+    return w;
+}
+
+// The next distinct adapter among the rows `todo`, its first row's lane in
+// lead; takes its rows out of todo.
 __device__ __forceinline__ int next_slot(const Tile& t, uint64_t& todo, int& lead) {
     lead = int(__builtin_ctzll(todo));
     const int s = __builtin_amdgcn_readlane(t.slot, lead);
     todo &= ~__ballot(t.slot == s);
     return s;
+}
+
+// An adapter that a tile names.
+struct Group {
+    uint64_t rows;   // its rows, a bit each
+    int slot;        // -1: the rows without an adapter
+    int rank;
+    float scale;
+};
+
+// The distinct adapters of the rows `of` to the LDS (one entry a row at
+// most); returns how many.  Ranks and scales are loaded for all rows at once.
+// All waves of the work-group come here with the same rows; a barrier at the
+// end.
+__device__ __forceinline__ int tile_groups(const LoraArgs& p, const Tile& t, uint64_t of, Group* out) {
+    const int at = max(t.slot, 0);
+    const int rank = p.rank[at];
+    const float scale = p.scale[at];
+    const Place w = tile_places(p, t, of);
+    if (w.first && threadIdx.x < kWave)
+        out[w.index] = Group{w.rows, t.slot, t.slot >= 0 ? min(max(rank, 0), p.R) : 0, scale};
+    __syncthreads();
+    return w.count;
+}
+// entry g, the same on every lane
+__device__ __forceinline__ Group group_at(const Group* groups, int g) {
+    const Group v = groups[g];
+    const uint32_t lo = __builtin_amdgcn_readfirstlane(uint32_t(v.rows)), hi = __builtin_amdgcn_readfirstlane(uint32_t(v.rows >> 32));
+    return Group{(uint64_t(hi) << 32) | lo, __builtin_amdgcn_readfirstlane(v.slot), __builtin_amdgcn_readfirstlane(v.rank),
+                 bits_f(__builtin_amdgcn_readfirstlane(f_bits(v.scale)))};
 }
 
 __device__ __forceinline__ void wave_sync_lds() {
@@ -208,15 +266,19 @@ __global__ __launch_bounds__(kShrinkWaves * kWave) void lora_shrink_kernel(LoraA
     const int chunk = blockIdx.z % chunks, item = blockIdx.z / chunks;
     const Tile t = tile_rows<kRows>(p, tile);
     uint64_t todo = __ballot(t.slot >= 0) & 0xFFFFu;
+    if (items > 1) {                                        // one of them, if there are as many
+        const Place w = tile_places(p, t, todo);
+        const uint64_t is = __ballot(w.first && w.index == item);
+        todo = is ? __builtin_amdgcn_readlane(uint32_t(w.rows), int(__builtin_ctzll(is))) : 0;
+    }
     // the split's steps [s0, s1), dealt to the waves in turn
     const int per = (ksteps + splits - 1) / splits;
     const int s0 = split * per + wave, s1 = min(ksteps, (split + 1) * per);
     const int r0 = chunk * NR * 16;
 
-    for (int it = 0; todo; ++it) {
+    while (todo) {
         int lead;
         const int slot = next_slot(t, todo, lead);
-        if (items > 1 && it != item) continue;
         const int rank = min(max(p.rank[slot], 0), p.R);
         const int nr = min(NR, (rank - r0 + 15) / 16);      // fragments with live ranks
         if (nr > 0) {
@@ -248,7 +310,6 @@ __global__ __launch_bounds__(kShrinkWaves * kWave) void lora_shrink_kernel(LoraA
             }
             __syncthreads();
         }
-        if (items > 1) break;
     }
 }
 
@@ -330,8 +391,8 @@ __device__ __forceinline__ int lds_row(int r) {        // -> its place: tile by 
 // without such rows (mask 0), which only bring B.  ZL: z of the wave's rows
 // lies in the LDS, in the workspace's order.
 template <bool GLU, int CC, bool HALF, bool BB, int NW, bool ZL>
-__device__ __forceinline__ void expand_cols(const LoraArgs& p, int splits, int slot, int rank, uint32_t mask,
-                                            int64_t row0, int first, int last, int width, u32x4* lds,
+__device__ __forceinline__ void expand_cols(const LoraArgs& p, int splits, int slot, int rank, float scale,
+                                            uint32_t mask, int64_t row0, int first, int last, int width, u32x4* lds,
                                             const f32x4* zl) {
     constexpr int kThreads = NW * kWave;
     constexpr int W = GLU ? 2 : 4, NP = GLU ? 2 : 1, C = CC ? CC : 1;
@@ -387,7 +448,6 @@ __device__ __forceinline__ void expand_cols(const LoraArgs& p, int splits, int s
     u32x4 zv[C][3];
     if constexpr (CC > 0) {
         if (mask) {
-            const float scale = p.scale[slot];
 #pragma unroll
             for (int c = 0; c < C; ++c) {
                 const int r = HALF ? (q & 1) * 8 : c * 32 + q * 8;
@@ -510,7 +570,7 @@ __global__ __launch_bounds__(kExpandWaves* kWave)
     LoraArgs p, int splits, int share, int nblocks) {
     constexpr int kMaxPitch = (MC == 0 ? 2 : MC == 1 ? 4 : 8) + 1;
     __shared__ u32x4 lds[2 * 64 * kMaxPitch];
-    const int wave = threadIdx.x / kWave, lane = threadIdx.x & (kWave - 1);
+    const int wave = threadIdx.x / kWave;
     // part by part over the tiles, the last ones first: those that a tile of
     // one adapter leaves unused end at once, on every XCD alike, and those of
     // tiles of two start before the others
@@ -522,14 +582,8 @@ __global__ __launch_bounds__(kExpandWaves* kWave)
     const int64_t row0 = int64_t(tile) * kExpandRows + wave * kRows;
     // rows without an adapter copy base, which in place is nothing to do
     const bool copy = GLU || p.base != p.y;
-    uint64_t todo = copy ? __ballot(t.in) : __ballot(t.slot >= 0);
-    int count = 0, slots = 0;                              // lane i: the i-th distinct adapter
-    while (todo) {
-        int lead;
-        const int slot = next_slot(t, todo, lead);
-        slots = lane == count ? slot : slots;
-        ++count;
-    }
+    __shared__ Group groups[kExpandRows];
+    const int count = tile_groups(p, t, copy ? __ballot(t.in) : __ballot(t.slot >= 0), groups);
     const int64_t total = int64_t(count) * blocks;
     const int64_t run = max(int64_t(nblocks), (total + share - 1) / share);
     int64_t at = part * run;
@@ -539,11 +593,11 @@ __global__ __launch_bounds__(kExpandWaves* kWave)
         const int n = int(min(end - at, int64_t(blocks - b0)));
         at += n;
         const int first = b0 * kBlock, last = min(width, first + n * kBlock);
-        const int slot = __builtin_amdgcn_readlane(slots, g);
-        const uint32_t mask = uint32_t(__ballot(t.in && t.slot == slot) >> (wave * kRows)) & 0xFFFFu;
-        const int rank = slot < 0 ? 0 : min(max(p.rank[slot], 0), p.R);
+        const Group gr = group_at(groups, g);
+        const int rank = gr.rank;
+        const uint32_t mask = uint32_t(gr.rows >> (wave * kRows)) & 0xFFFFu;
 #define GRIM_COLS(CC, HALF) \
-    expand_cols<GLU, CC, HALF, BB, kExpandWaves, false>(p, splits, slot, rank, mask, row0, first, last, width, lds, nullptr)
+    expand_cols<GLU, CC, HALF, BB, kExpandWaves, false>(p, splits, gr.slot, rank, gr.scale, mask, row0, first, last, width, lds, nullptr)
         if (rank == 0) {
             if (copy) GRIM_COLS(0, false);
         } else if constexpr (MC == 0) {
@@ -579,14 +633,8 @@ __global__ __launch_bounds__(kShrinkWaves* kWave) void lora_one_kernel(LoraArgs 
     const int blocks = (width + kBlock - 1) / kBlock, ksteps = (p.K + kStep - 1) / kStep;
     const Tile t = tile_rows<kRows>(p, 0);
     const bool copy = GLU || p.base != p.y;
-    uint64_t todo = (copy ? __ballot(t.in) : __ballot(t.slot >= 0)) & 0xFFFFu;
-    int count = 0, slots = 0;
-    while (todo) {
-        int lead;
-        const int slot = next_slot(t, todo, lead);
-        slots = lane == count ? slot : slots;
-        ++count;
-    }
+    __shared__ Group groups[kRows];
+    const int count = tile_groups(p, t, (copy ? __ballot(t.in) : __ballot(t.slot >= 0)) & 0xFFFFu, groups);
     const int total = count * blocks, run = (total + share - 1) / share;
     int at = int(blockIdx.x) * run;
     const int end = min(total, at + run);
@@ -594,16 +642,15 @@ __global__ __launch_bounds__(kShrinkWaves* kWave) void lora_one_kernel(LoraArgs 
         const int g = at / blocks, b0 = at - g * blocks, n = min(end - at, blocks - b0);
         at += n;
         const int first = b0 * kBlock, last = min(width, first + n * kBlock);
-        const int slot = __builtin_amdgcn_readlane(slots, g);
-        const uint32_t mask = uint32_t(__ballot(t.in && t.slot == slot)) & 0xFFFFu;
-        const int rank = slot < 0 ? 0 : min(max(p.rank[slot], 0), p.R);
+        const Group gr = group_at(groups, g);
+        const int rank = gr.rank;
+        const uint32_t mask = uint32_t(gr.rows);
         const int nr = min(NR, (rank + 15) / 16);
         if (nr > 0) {
             f32x4 acc[4] = {};
             int ln = lane;                                  // opaque: see expand_cols
             asm volatile("" : "+v"(ln));
-            const int lead = __builtin_ctz(mask);
-#define GRIM_STEPS(NF) shrink_steps<XB, NF>(p, slot, 0, mask, 0, lead, ln, wave, ksteps, lds[wave], acc)
+#define GRIM_STEPS(NF) shrink_steps<XB, NF>(p, gr.slot, 0, mask, 0, __builtin_ctz(mask), ln, wave, ksteps, lds[wave], acc)
             if (NR == 1 || nr == 1) GRIM_STEPS(1);
             else if (NR == 2 || nr == 2) GRIM_STEPS(2);
             else GRIM_STEPS(4);
@@ -626,7 +673,7 @@ __global__ __launch_bounds__(kShrinkWaves* kWave) void lora_one_kernel(LoraArgs 
         }
         const uint32_t mine = wave == 0 ? mask : 0;
 #define GRIM_COLS(CC, HALF) \
-    expand_cols<GLU, CC, HALF, BB, kShrinkWaves, true>(p, 1, slot, rank, mine, 0, first, last, width, lds[0], zl)
+    expand_cols<GLU, CC, HALF, BB, kShrinkWaves, true>(p, 1, gr.slot, rank, gr.scale, mine, 0, first, last, width, lds[0], zl)
         if (rank == 0) {
             if (copy) GRIM_COLS(0, false);
         } else if constexpr (MC == 0) {
@@ -673,7 +720,7 @@ void shrink(hipStream_t st, const LoraArgs& a, int splits, int items) {
 // every tile is one adapter's, which leaves room for the tiles of two (4096
 // rows of 9 requests, 2048 -> 7168: 34.8 us; runs that fill the chip: 40.4);
 // three of them share out tiles of many (48 mixed rows of 32 adapters:
-// 12.2 us against 15 with two or four).
+// 15.7 us in all; with two or four 18.4, 17.0).
 constexpr int kExpandRuns = 512, kExpandGroups = 768;
 
 template <bool GLU, bool BB>
