@@ -92,7 +92,7 @@ __device__ __forceinline__ Tile tile_rows(const LoraArgs& p, int tile) {
 // Where this lane's row stands among the distinct adapters that the rows `of`
 // name (no adapter counts as one more), in the order of their first rows.
 // Equal slots are found by a ballot a bit of their numbers, so that 64
-// adapters cost what two do (48 mixed rows of 32 adapters, 2048 -> 7168: 15.7
+// adapters cost what two do (48 mixed rows of 32 adapters, 2048 -> 7168: 15.4
 // us; counted one after the other 17.7).
 struct Place {
     uint64_t rows;   // the rows of its adapter, a bit each
@@ -564,9 +564,11 @@ __device__ __forceinline__ void expand_cols(const LoraArgs& p, int splits, int s
 // adapter by adapter; `share` work-groups split it evenly into runs of at
 // least nblocks.  How many adapters a tile names is known here only: one for
 // most tiles of a prompt, dozens for sequences decoding together.
+// (Rank 64 in 3 waves a SIMD, without spills: 48 mixed rows 15.4 us, in 4
+// 15.7; long batches alike.)
 template <bool GLU, int MC, bool BB>
 __global__ __launch_bounds__(kExpandWaves* kWave)
-    __attribute__((amdgpu_waves_per_eu(MC > 2 ? 2 : 4))) void lora_expand_kernel(
+    __attribute__((amdgpu_waves_per_eu(MC > 2 ? 2 : 3))) void lora_expand_kernel(
     LoraArgs p, int splits, int share, int nblocks) {
     constexpr int kMaxPitch = (MC == 0 ? 2 : MC == 1 ? 4 : 8) + 1;
     __shared__ u32x4 lds[2 * 64 * kMaxPitch];
@@ -716,11 +718,11 @@ void shrink(hipStream_t st, const LoraArgs& a, int splits, int items) {
 #undef GRIM_SHRINK
 }
 
-// expand's work-groups, 4 a CU at once: runs of blocks of two of them while
+// expand's work-groups, 3 or 4 a CU at once: runs of blocks of two of them while
 // every tile is one adapter's, which leaves room for the tiles of two (4096
 // rows of 9 requests, 2048 -> 7168: 34.8 us; runs that fill the chip: 40.4);
 // three of them share out tiles of many (48 mixed rows of 32 adapters:
-// 15.7 us in all; with two or four 18.4, 17.0).
+// 15.4 us in all; with two or four 18.4, 17.0).
 constexpr int kExpandRuns = 512, kExpandGroups = 768;
 
 template <bool GLU, bool BB>

@@ -273,3 +273,20 @@ def test_loading_and_refusals(gpu):
             lora.add(**kw)
     with pytest.raises(_abi.GrimoireError):
         lora.swiglu(slot, x, y, y)
+
+
+@pytest.mark.parametrize("slots", [2, 255, 256, 1000])
+def test_many_slots(gpu, slots):
+    """Tiles of dozens of adapters whose slots share most bits, short and
+    long batches, the last slot and rows without one among them."""
+    for T in (16, 64, 530):
+        d = make(T, 64, 72, slots, 16, 60 + slots)
+        d["slot"][: min(T, 12)] = torch.tensor([slots - 1, -1, slots - 2, 0, slots - 1, slots, slots // 2,
+                                                slots // 2 - 1, -1, 1, 2**31 - 1, -2**31], dtype=torch.int32)
+        e = dict(d, slot=torch.where((d["slot"] < 0) | (d["slot"] >= slots), -1, d["slot"]))
+        ad = weights.LoraAdapters(*(d[k].to(gpu) for k in ("a", "b", "rank", "scale")))
+        y = torch.full((T, 72), float("nan"), device=gpu)
+        ops.Lora(ad, T).add(d["slot"].to(gpu), d["x"].to(gpu), y, base=d["base"].to(gpu))
+        torch.cuda.synchronize()
+        v, tol = want(e)
+        assert ((y.cpu().double() - v).abs() <= tol).all()
