@@ -419,7 +419,10 @@ class BlockNorm:
                 _dev(w)
                 _flat(w, "norm weight", (w.numel(),), _B16, w.get_device())
         self._pre, self._post, self._gate = pre_weight, post_weight, gate
-        self._weights_of = {(w.numel(), w.get_device()) for w in (pre_weight, post_weight) if w is not None}
+        of = {(w.numel(), w.get_device()) for w in (pre_weight, post_weight) if w is not None}
+        if len(of) > 1:
+            raise _abi.GrimoireError("norm weights of different lengths or devices")
+        self._weights_of = of.pop() if of else None
         self._dense, self._moe = lib().grimoire_block_norm, lib().grimoire_moe_block_norm
         self.struct = _abi.BlockNormParams(_p(post_weight), _p(pre_weight), float(weight_offset), float(eps),
                                            float(residual_scale), float(block_scale), self.GATES[gate],
@@ -436,9 +439,8 @@ class BlockNorm:
         if h.dim() != 2:
             raise _abi.GrimoireError("h: [T][H]")
         T, H = shape = h.shape
-        for of in self._weights_of:
-            if of != (H, dev):
-                raise _abi.GrimoireError("norm weights: one value a column, on h's device")
+        if self._weights_of is not None and self._weights_of != (H, dev):
+            raise _abi.GrimoireError("norm weights: one value a column, on h's device")
         kind = self._gate
         if (gate is not None) != (kind != "none"):
             raise _abi.GrimoireError(f"gate {kind!r} and the gate tensor do not go together")
@@ -489,14 +491,14 @@ class Lora:
         self.max_rows = max_rows
         self.dev = adapters.a.get_device()
         nbytes = int(lib().grimoire_lora_workspace_bytes(self.struct, max_rows))
-        self.workspace = torch.empty(nbytes, dtype=torch.uint8, device=adapters.a.device)
-        self._ref = C.byref(self.struct)
+        self._workspace = torch.empty(nbytes, dtype=torch.uint8, device=adapters.a.device)
+        self._ref, self._ws = C.byref(self.struct), (self._workspace.data_ptr(), nbytes)
         self._add, self._swiglu = lib().grimoire_lora_add, lib().grimoire_lora_swiglu
 
     adapters = property(lambda self: self._adapters)
+    workspace = property(lambda self: self._workspace)
 
     def _call(self, fn, what, row_slot, x, base, y, width, stream):
-        _gpu(x)
         (K, N), dev = self._KN, self.dev
         if x.dim() != 2:
             raise _abi.GrimoireError("x: [T][K]")
@@ -509,7 +511,7 @@ class Lora:
         bp, b16, bs = _rows(base, "base", N, T)
         yp, y16, ys = _rows(y, "output", width, T)
         _launch(dev, stream, fn, what, self._ref, _flat(row_slot, "row_slot", (T,), _I32, dev), xp, x16, xs, bp, b16,
-                bs, yp, y16, ys, T, self.workspace.data_ptr(), self.workspace.numel())
+                bs, yp, y16, ys, T, *self._ws)
 
     def add(self, row_slot, x, y, base=None, stream=None):
         """y = base + the adapters' product of x (base None: y += it).

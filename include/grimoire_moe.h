@@ -369,7 +369,9 @@ int grimoire_rmsnorm_residual(void* stream, float* h, const float* r0, const flo
  * (either may be NULL; without both, pre_weight may be NULL).  The norm
  * weights are bf16 [hidden].  hidden % 4 == 0, <= 32768; fp32 rows 16-byte,
  * bf16 rows 8-byte aligned.  An output may take the place of an input of its
- * own type and row distance; it overlaps nothing else.
+ * own type and row distance; it overlaps nothing else.  Sums are fp32; up to
+ * 256 rows they are spread over more threads, so the last bits of a row may
+ * differ from those it has in a larger batch.
  *   grimoire_block_norm: f = x[t], fp32 or (x_bf16) bf16 rows x_stride
  *     elements apart (a multiple of 4, >= hidden).
  *   grimoire_moe_block_norm: f = shared[t] (fp32, may be NULL) + sum_s
