@@ -32,14 +32,10 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 
-constexpr int kRows = 16;        // rows of a tile
-constexpr int kStep = 64;        // shrink: k of one step of a wave, 16 a lane
-constexpr int kShrinkWaves = 8;
+constexpr int kRows = kLoraRows;
+constexpr int kStep = kLoraStep;     // 16 k a lane
+constexpr int kShrinkWaves = kLoraShrinkWaves;
 constexpr int kExpandWaves = 4;
-// shrink: batches of up to this many rows give every distinct adapter of a
-// tile a work-group of its own.
-constexpr int kItemRows = 512;
-constexpr int kMaxSplits = 8;
 
 __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
     bf16x8 av, bv;
@@ -162,15 +158,12 @@ __device__ __forceinline__ void wave_sync_lds() {
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
-// The workspace holds z as expand's operands: per split, tile of 16 rows and
-// 32 ranks two runs of 64 lanes' four values; expand's lane (q, col) takes
+// Of a chunk's two runs of z in the workspace expand's lane (q, col) takes
 // ranks 8 q .. 8 q + 3 of row col from the first, the next four from the
 // second.  This is where shrink's lane (q, col), with ranks 4 q .. 4 q + 3 of
 // fragment f, puts its own.
 __device__ __forceinline__ f32x4* z_run(const LoraArgs& p, int split, int64_t tile, int chunk, int half) {
-    const int chunks = (p.R + 31) / 32;
-    const int64_t tiles = (p.T + kRows - 1) / kRows;
-    return reinterpret_cast<f32x4*>(p.part) + (((split * tiles + tile) * chunks + chunk) * 2 + half) * kWave;
+    return reinterpret_cast<f32x4*>(p.part) + lora_z_run(p.R, p.T, split, tile, chunk, half) * kWave;
 }
 __device__ __forceinline__ f32x4* z_at(const LoraArgs& p, int split, int64_t tile, int f, int q, int col) {
     return z_run(p, split, tile, f >> 1, q & 1) + ((f & 1) * 2 + (q >> 1)) * 16 + col;
@@ -458,7 +451,7 @@ __device__ __forceinline__ void expand_cols(const LoraArgs& p, int splits, int s
                     hi = zl[(c * 2 + 1) * kWave + at];
                 } else {
                     const int64_t apart = z_run(p, 1, 0, 0, 0) - z_run(p, 0, 0, 0, 0);
-                    const f32x4* z0 = z_run(p, 0, row0 / kRows, c, 0) + at;
+                    const f32x4* z0 = z_run(p, 0, row0 / kRows, lora_z_chunk(p.R, c), 0) + at;
                     for (int s = 0; s < splits; s += 2) {
                         const f32x4* z1 = z0 + s * apart;
                         const f32x4* z2 = z0 + min(s + 1, splits - 1) * apart;
@@ -605,9 +598,10 @@ __global__ __launch_bounds__(kExpandWaves* kWave)
         } else if constexpr (MC == 0) {
             GRIM_COLS(1, true);
         } else {
-            if (MC == 1 || rank <= 32) GRIM_COLS(1, false);
-            else if (MC == 2 || rank <= 64) GRIM_COLS((MC < 2 ? MC : 2), false);
-            else if (MC == 4 || rank <= 128) GRIM_COLS((MC < 4 ? MC : 4), false);
+            const int code = lora_code_chunks(MC, rank);
+            if (code == 1) GRIM_COLS(1, false);
+            else if (code == 2) GRIM_COLS((MC < 2 ? MC : 2), false);
+            else if (code == 4) GRIM_COLS((MC < 4 ? MC : 4), false);
             else GRIM_COLS(MC, false);
         }
 #undef GRIM_COLS
@@ -689,20 +683,6 @@ __global__ __launch_bounds__(kShrinkWaves* kWave) void lora_one_kernel(LoraArgs 
     }
 }
 
-// K splits over work-groups: as many as leave each wave one step, for short
-// batches; long ones take as many of these as make two work-groups a CU.
-int short_splits(int K) {
-    const int ksteps = (K + kStep - 1) / kStep, s = (ksteps + kShrinkWaves - 1) / kShrinkWaves;
-    return s > kMaxSplits ? kMaxSplits : s;
-}
-constexpr int kShrinkGroups = 512;
-int lora_splits(int K, int T) {
-    const int s = short_splits(K);
-    if (T <= kItemRows) return s;
-    const int tiles = (T + kRows - 1) / kRows, w = (kShrinkGroups + tiles - 1) / tiles;
-    return s < w ? s : w;
-}
-
 template <bool XB>
 void shrink(hipStream_t st, const LoraArgs& a, int splits, int items) {
     const int tiles = (a.T + kRows - 1) / kRows, ksteps = (a.K + kStep - 1) / kStep;
@@ -740,9 +720,9 @@ void expand(hipStream_t st, const LoraArgs& a, int splits) {
 #define GRIM_EXPAND(MC) \
     hipLaunchKernelGGL((lora_expand_kernel<GLU, MC, BB>), grid, dim3(kExpandWaves * kWave), 0, st, a, splits, int(share), nb)
     if (a.R <= 16) GRIM_EXPAND(0);
-    else if (a.R <= 32) GRIM_EXPAND(1);
-    else if (a.R <= 64) GRIM_EXPAND(2);
-    else if (a.R <= 128) GRIM_EXPAND(4);
+    else if (lora_max_chunks(a.R) == 1) GRIM_EXPAND(1);
+    else if (lora_max_chunks(a.R) == 2) GRIM_EXPAND(2);
+    else if (lora_max_chunks(a.R) == 4) GRIM_EXPAND(4);
     else GRIM_EXPAND(8);
 #undef GRIM_EXPAND
 }
@@ -780,14 +760,6 @@ void one(hipStream_t st, const LoraArgs& a, int groups) {
 
 }  // namespace
 
-size_t lora_workspace_bytes(int K, int R, int T) {
-    if (K <= 0 || R <= 0 || T <= 0) return 0;
-    // for up to T rows: splits * rows is at most this for every shorter batch
-    const size_t rows = (size_t(T) + kRows - 1) / kRows * kRows, most = short_splits(K) * rows;
-    const size_t lng = size_t(kShrinkGroups) * kRows + rows;
-    return (most < lng || T <= kItemRows ? most : lng) * ((R + 31) / 32 * 32) * sizeof(float);
-}
-
 hipError_t lora_launch(hipStream_t st, const LoraArgs& a) {
     if (a.T <= 0) return hipSuccess;
     if (const int groups = one_groups(a)) {
@@ -797,7 +769,7 @@ hipError_t lora_launch(hipStream_t st, const LoraArgs& a) {
     }
     const int splits = lora_splits(a.K, a.T);
     // distinct adapters a tile can name, rows without one among them
-    const int items = a.T > kItemRows ? 1 : a.T < kRows ? a.T : kRows;
+    const int items = a.T > kLoraItemRows ? 1 : a.T < kRows ? a.T : kRows;
     if (a.x_bf16) shrink<true>(st, a, splits, items);
     else shrink<false>(st, a, splits, items);
     hipError_t e = hipGetLastError();

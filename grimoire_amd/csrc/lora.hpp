@@ -2,6 +2,7 @@
 #pragma once
 
 #include "common.hpp"
+#include "lora_layout.hpp"
 
 namespace grim {
 
@@ -26,7 +27,6 @@ struct LoraArgs {
 constexpr int kLoraMaxRank = 256;
 constexpr int64_t kLoraMaxStride = int64_t(1) << 24;
 
-size_t lora_workspace_bytes(int K, int R, int T);
 hipError_t lora_launch(hipStream_t st, const LoraArgs& a);
 
 }  // namespace grim

@@ -1,0 +1,69 @@
+// lora_layout.hpp -- where z = A x lies between the adapters' two launches,
+// and which of it expand reads.  Integers alone, for the kernels and for host
+// code that follows their indexes.
+//
+// The workspace holds z as expand's operands: per K split, tile of 16 rows
+// and chunk of 32 ranks (those of max_rank, no more) two runs of 64 lanes'
+// four fp32 values.
+#pragma once
+
+#include <stddef.h>
+#include <stdint.h>
+
+#ifdef __HIPCC__
+#define GRIM_HD __host__ __device__
+#else
+#define GRIM_HD
+#endif
+
+namespace grim {
+
+constexpr int kLoraRows = 16;          // rows of a tile
+constexpr int kLoraStep = 64;          // shrink: k of one step of a wave
+constexpr int kLoraShrinkWaves = 8;
+// shrink: batches of up to this many rows give every distinct adapter of a
+// tile a work-group of its own.
+constexpr int kLoraItemRows = 512;
+constexpr int kLoraMaxSplits = 8;
+constexpr int kLoraShrinkGroups = 512;
+constexpr int kLoraRunBytes = 64 * 16;
+
+// K splits over work-groups: as many as leave each wave one step, for short
+// batches; long ones take as many of these as make two work-groups a CU.
+constexpr int lora_short_splits(int K) {
+    const int ksteps = (K + kLoraStep - 1) / kLoraStep, s = (ksteps + kLoraShrinkWaves - 1) / kLoraShrinkWaves;
+    return s > kLoraMaxSplits ? kLoraMaxSplits : s;
+}
+constexpr int lora_splits(int K, int T) {
+    const int s = lora_short_splits(K);
+    if (T <= kLoraItemRows) return s;
+    const int tiles = (T - 1) / kLoraRows + 1, w = (kLoraShrinkGroups + tiles - 1) / tiles;
+    return s < w ? s : w;
+}
+
+GRIM_HD constexpr int lora_z_chunks(int R) { return (R + 31) / 32; }
+// run `half` of a split's, tile's and chunk's z, counted in runs
+GRIM_HD constexpr int64_t lora_z_run(int R, int T, int split, int64_t tile, int chunk, int half) {
+    const int64_t tiles = (int64_t(T) + kLoraRows - 1) / kLoraRows;
+    return ((split * tiles + tile) * lora_z_chunks(R) + chunk) * 2 + half;
+}
+constexpr size_t lora_workspace_bytes(int K, int R, int T) {
+    if (K <= 0 || R <= 0 || T <= 0) return 0;
+    // for up to T rows: splits * rows is at most this for every shorter batch
+    const size_t rows = (size_t(T) + kLoraRows - 1) / kLoraRows * kLoraRows, most = lora_short_splits(K) * rows;
+    const size_t lng = size_t(kLoraShrinkGroups) * kLoraRows + rows;
+    return (most < lng || T <= kLoraItemRows ? most : lng) * (lora_z_chunks(R) * 32) * sizeof(float);
+}
+
+// expand has code for 1, 2, 4 and 8 chunks.  mc: those of max_rank's kernel;
+// an adapter takes the code of its own rank.
+GRIM_HD constexpr int lora_max_chunks(int R) { return R <= 32 ? 1 : R <= 64 ? 2 : R <= 128 ? 4 : 8; }
+GRIM_HD constexpr int lora_code_chunks(int mc, int rank) {
+    return mc <= 1 || rank <= 32 ? 1 : mc == 2 || rank <= 64 ? 2 : mc == 4 || rank <= 128 ? 4 : 8;
+}
+// Which chunk of z that code reads for its chunk c: a chunk past max_rank's
+// (rank 65 to 96 of a max_rank 80 or 96 takes the code of four, where the
+// workspace holds three) reads the last there is, under a z of zero.
+GRIM_HD constexpr int lora_z_chunk(int R, int c) { return c < lora_z_chunks(R) ? c : lora_z_chunks(R) - 1; }
+
+}  // namespace grim
