@@ -446,12 +446,14 @@ __device__ __forceinline__ void expand_cols(const LoraArgs& p, int splits, int s
                 const int r = HALF ? (q & 1) * 8 : c * 32 + q * 8;
                 const int at = HALF ? lane & 31 : lane;
                 f32x4 lo = {}, hi = {};
-                if constexpr (ZL) {
+                if (!lora_z_read(C, rank, c)) {
+                    // no live rank: z is zero
+                } else if constexpr (ZL) {
                     lo = zl[c * 2 * kWave + at];
                     hi = zl[(c * 2 + 1) * kWave + at];
                 } else {
                     const int64_t apart = z_run(p, 1, 0, 0, 0) - z_run(p, 0, 0, 0, 0);
-                    const f32x4* z0 = z_run(p, 0, row0 / kRows, lora_z_chunk(p.R, c), 0) + at;
+                    const f32x4* z0 = z_run(p, 0, row0 / kRows, c, 0) + at;
                     for (int s = 0; s < splits; s += 2) {
                         const f32x4* z1 = z0 + s * apart;
                         const f32x4* z2 = z0 + min(s + 1, splits - 1) * apart;

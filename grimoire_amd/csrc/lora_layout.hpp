@@ -61,9 +61,11 @@ GRIM_HD constexpr int lora_max_chunks(int R) { return R <= 32 ? 1 : R <= 64 ? 2 
 GRIM_HD constexpr int lora_code_chunks(int mc, int rank) {
     return mc <= 1 || rank <= 32 ? 1 : mc == 2 || rank <= 64 ? 2 : mc == 4 || rank <= 128 ? 4 : 8;
 }
-// Which chunk of z that code reads for its chunk c: a chunk past max_rank's
-// (rank 65 to 96 of a max_rank 80 or 96 takes the code of four, where the
-// workspace holds three) reads the last there is, under a z of zero.
-GRIM_HD constexpr int lora_z_chunk(int R, int c) { return c < lora_z_chunks(R) ? c : lora_z_chunks(R) - 1; }
+// Whether the code of `code` chunks reads chunk c of z: where the adapter has
+// a rank in it.  The code was chosen by the rank, which reaches into the first
+// code / 2 + 1 of its chunks (known when compiling); the ones behind may lie
+// past max_rank's too: rank 65 to 96 of a max_rank 80 or 96 takes the code of
+// four, where the workspace holds three.
+GRIM_HD constexpr bool lora_z_read(int code, int rank, int c) { return c <= code / 2 || c * 32 < rank; }
 
 }  // namespace grim

@@ -1,7 +1,7 @@
 """Every index of the adapter kernels' workspace, followed on the host from the
 functions that the kernels themselves use: z as it is written and as expand
 reads it lies within grimoire_lora_workspace_bytes for every max_rank, rank,
-split and number of rows, and a live rank is read from its own chunk."""
+split and number of rows, and every live rank is read."""
 import ctypes as C
 import os
 import subprocess
@@ -16,7 +16,7 @@ PROGRAM = r"""
 using namespace grim;
 
 // end of the last byte of z that shrink writes (at[0]) and expand reads
-// (at[1]) for `rows` rows; 1 if a live rank is read from another chunk
+// (at[1]) for `rows` rows; 1 if a live rank is not read
 extern "C" int z_ends(int K, int R, int rows, int64_t* at) {
     const int splits = lora_splits(K, rows), mc = lora_max_chunks(R);
     const int64_t tiles = (int64_t(rows) + kLoraRows - 1) / kLoraRows;
@@ -27,9 +27,12 @@ extern "C" int z_ends(int K, int R, int rows, int64_t* at) {
         const int code = lora_code_chunks(mc, rank);
         if (code * 32 < rank) return 1;
         for (int c = 0; c < code; ++c) {
-            const int z = lora_z_chunk(R, c);
-            if (z < 0 || (c * 32 < rank && z != c)) return 1;
-            at[1] = std::max(at[1], (lora_z_run(R, rows, splits - 1, tiles - 1, z, 1) + 1) * kLoraRunBytes);
+            const bool live = c * 32 < rank;
+            if (!lora_z_read(code, rank, c)) {
+                if (live) return 1;
+                continue;
+            }
+            at[1] = std::max(at[1], (lora_z_run(R, rows, splits - 1, tiles - 1, c, 1) + 1) * kLoraRunBytes);
         }
     }
     return 0;
