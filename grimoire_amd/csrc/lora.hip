@@ -446,9 +446,7 @@ __device__ __forceinline__ void expand_cols(const LoraArgs& p, int splits, int s
                 const int r = HALF ? (q & 1) * 8 : c * 32 + q * 8;
                 const int at = HALF ? lane & 31 : lane;
                 f32x4 lo = {}, hi = {};
-                if (!lora_z_read(C, rank, c)) {
-                    // no live rank: z is zero
-                } else if constexpr (ZL) {
+                if constexpr (ZL) {
                     lo = zl[c * 2 * kWave + at];
                     hi = zl[(c * 2 + 1) * kWave + at];
                 } else {
@@ -600,10 +598,9 @@ __global__ __launch_bounds__(kExpandWaves* kWave)
         } else if constexpr (MC == 0) {
             GRIM_COLS(1, true);
         } else {
-            const int code = lora_code_chunks(MC, rank);
-            if (code == 1) GRIM_COLS(1, false);
-            else if (code == 2) GRIM_COLS((MC < 2 ? MC : 2), false);
-            else if (code == 4) GRIM_COLS((MC < 4 ? MC : 4), false);
+            if (lora_code_is(1, MC, rank)) GRIM_COLS(1, false);
+            else if (lora_code_is(2, MC, rank)) GRIM_COLS((MC < 2 ? MC : 2), false);
+            else if (lora_code_is(4, MC, rank)) GRIM_COLS((MC < 4 ? MC : 4), false);
             else GRIM_COLS(MC, false);
         }
 #undef GRIM_COLS

@@ -3,8 +3,8 @@
 // code that follows their indexes.
 //
 // The workspace holds z as expand's operands: per K split, tile of 16 rows
-// and chunk of 32 ranks (those of max_rank, no more) two runs of 64 lanes'
-// four fp32 values.
+// and chunk of 32 ranks two runs of 64 lanes' four fp32 values, as many chunks
+// as expand's code for max_rank reads (max_rank 80 or 96: four).
 #pragma once
 
 #include <stddef.h>
@@ -41,31 +41,23 @@ constexpr int lora_splits(int K, int T) {
     return s < w ? s : w;
 }
 
-GRIM_HD constexpr int lora_z_chunks(int R) { return (R + 31) / 32; }
+// expand has code for 1, 2, 4 and 8 chunks of 32 ranks.  mc: the most that
+// max_rank's kernel has; an adapter takes the first code that holds its rank,
+// which reads all of its chunks of z, live ranks in them or not.
+GRIM_HD constexpr int lora_max_chunks(int R) { return R <= 32 ? 1 : R <= 64 ? 2 : R <= 128 ? 4 : 8; }
+GRIM_HD constexpr bool lora_code_is(int chunks, int mc, int rank) { return mc <= chunks || rank <= chunks * 32; }
+
 // run `half` of a split's, tile's and chunk's z, counted in runs
 GRIM_HD constexpr int64_t lora_z_run(int R, int T, int split, int64_t tile, int chunk, int half) {
-    const int64_t tiles = (int64_t(T) + kLoraRows - 1) / kLoraRows;
-    return ((split * tiles + tile) * lora_z_chunks(R) + chunk) * 2 + half;
+    const int64_t tiles = (T + kLoraRows - 1) / kLoraRows;
+    return ((split * tiles + tile) * lora_max_chunks(R) + chunk) * 2 + half;
 }
 constexpr size_t lora_workspace_bytes(int K, int R, int T) {
     if (K <= 0 || R <= 0 || T <= 0) return 0;
     // for up to T rows: splits * rows is at most this for every shorter batch
     const size_t rows = (size_t(T) + kLoraRows - 1) / kLoraRows * kLoraRows, most = lora_short_splits(K) * rows;
     const size_t lng = size_t(kLoraShrinkGroups) * kLoraRows + rows;
-    return (most < lng || T <= kLoraItemRows ? most : lng) * (lora_z_chunks(R) * 32) * sizeof(float);
+    return (most < lng || T <= kLoraItemRows ? most : lng) * (lora_max_chunks(R) * 32) * sizeof(float);
 }
-
-// expand has code for 1, 2, 4 and 8 chunks.  mc: those of max_rank's kernel;
-// an adapter takes the code of its own rank.
-GRIM_HD constexpr int lora_max_chunks(int R) { return R <= 32 ? 1 : R <= 64 ? 2 : R <= 128 ? 4 : 8; }
-GRIM_HD constexpr int lora_code_chunks(int mc, int rank) {
-    return mc <= 1 || rank <= 32 ? 1 : mc == 2 || rank <= 64 ? 2 : mc == 4 || rank <= 128 ? 4 : 8;
-}
-// Whether the code of `code` chunks reads chunk c of z: where the adapter has
-// a rank in it.  The code was chosen by the rank, which reaches into the first
-// code / 2 + 1 of its chunks (known when compiling); the ones behind may lie
-// past max_rank's too: rank 65 to 96 of a max_rank 80 or 96 takes the code of
-// four, where the workspace holds three.
-GRIM_HD constexpr bool lora_z_read(int code, int rank, int c) { return c <= code / 2 || c * 32 < rank; }
 
 }  // namespace grim

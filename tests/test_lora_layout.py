@@ -1,7 +1,7 @@
 """Every index of the adapter kernels' workspace, followed on the host from the
 functions that the kernels themselves use: z as it is written and as expand
 reads it lies within grimoire_lora_workspace_bytes for every max_rank, rank,
-split and number of rows, and every live rank is read."""
+split and number of rows."""
 import ctypes as C
 import os
 import subprocess
@@ -16,7 +16,7 @@ PROGRAM = r"""
 using namespace grim;
 
 // end of the last byte of z that shrink writes (at[0]) and expand reads
-// (at[1]) for `rows` rows; 1 if a live rank is not read
+// (at[1]) for `rows` rows; 1 if a rank's code is too short
 extern "C" int z_ends(int K, int R, int rows, int64_t* at) {
     const int splits = lora_splits(K, rows), mc = lora_max_chunks(R);
     const int64_t tiles = (int64_t(rows) + kLoraRows - 1) / kLoraRows;
@@ -24,16 +24,11 @@ extern "C" int z_ends(int K, int R, int rows, int64_t* at) {
     for (int rank = 1; rank <= R; ++rank) {
         for (int f = 0; f < (rank + 15) / 16; ++f)
             at[0] = std::max(at[0], (lora_z_run(R, rows, splits - 1, tiles - 1, f >> 1, 1) + 1) * kLoraRunBytes);
-        const int code = lora_code_chunks(mc, rank);
+        int code = 1;
+        while (!lora_code_is(code, mc, rank)) code *= 2;
         if (code * 32 < rank) return 1;
-        for (int c = 0; c < code; ++c) {
-            const bool live = c * 32 < rank;
-            if (!lora_z_read(code, rank, c)) {
-                if (live) return 1;
-                continue;
-            }
+        for (int c = 0; c < code; ++c)
             at[1] = std::max(at[1], (lora_z_run(R, rows, splits - 1, tiles - 1, c, 1) + 1) * kLoraRunBytes);
-        }
     }
     return 0;
 }
