@@ -310,7 +310,7 @@ static bool share_memory(const RowSpan& a, const RowSpan& b) {
     return d < a.width || d + b.width > a.stride;
 }
 static bool same_rows(const RowSpan& a, const RowSpan& b) {
-    return a.p == b.p && a.stride == b.stride && a.width == b.width;
+    return a.p == b.p && a.stride == b.stride && a.width == b.width && a.rows == b.rows;
 }
 
 int grimoire_moe_router_scores(void* stream, const grim_score_params* p, const void* logits,
@@ -499,14 +499,19 @@ int grimoire_rmsnorm_residual(void* stream, float* h, const float* r0, const flo
     return status(combine_norm_launch(S(stream), a));
 }
 
-// An output of a block norm may take the place of an input of its own layout
-// (each row is read before it is written) and overlaps nothing else.
-static bool norm_overlap(const BlockNormArgs& a, std::initializer_list<RowSpan> inputs) {
+// An output of a block norm may take the place of one of the inputs `rows`, of
+// its own type, distance and number of rows (each row is read before it is
+// written, by the work-group that writes it), and overlaps nothing else: of
+// `whole` any row may read any part.
+static bool norm_overlap(const BlockNormArgs& a, std::initializer_list<RowSpan> rows,
+                         std::initializer_list<RowSpan> whole) {
     const int64_t f = int64_t(a.H) * 4, b = int64_t(a.H) * 2;
     const RowSpan outs[3] = {{a.h_out, f, f, a.T}, {a.out, f, f, a.T}, {a.out_bf, b, b, a.T}};
     for (int i = 0; i < 3; ++i) {
-        for (const RowSpan& in : inputs)
+        for (const RowSpan& in : rows)
             if (share_memory(outs[i], in) && !same_rows(outs[i], in)) return true;
+        for (const RowSpan& in : whole)
+            if (share_memory(outs[i], in)) return true;
         for (int j = 0; j < i; ++j)
             if (share_memory(outs[i], outs[j])) return true;
     }
@@ -559,7 +564,7 @@ int grimoire_block_norm(void* stream, const grim_block_norm_params* p, const voi
     if (!aligned(x, x_bf16 ? 8 : 16)) return fail(GRIM_ERR_ARG, "x alignment");
     a.x = x; a.x_bf16 = x_bf16 ? 1 : 0; a.x_stride = x_stride;
     const int64_t size = x_bf16 ? 2 : 4, row = int64_t(hidden) * 4;
-    if (norm_overlap(a, {{h, row, row, tokens}, {x, x_stride * size, hidden * size, tokens}, gate_span(a)}))
+    if (norm_overlap(a, {{h, row, row, tokens}, {x, x_stride * size, hidden * size, tokens}, gate_span(a)}, {}))
         return fail(GRIM_ERR_ARG, "an output overlaps another argument");
     return status(block_norm_launch(S(stream), a));
 }
@@ -576,9 +581,12 @@ int grimoire_moe_block_norm(void* stream, const grim_block_norm_params* p, const
     if (routed_rows < 0) return fail(GRIM_ERR_SHAPE, "routed_rows=%d", routed_rows);
     if (!aligned(routed, 8) || !aligned(shared, 16)) return fail(GRIM_ERR_ARG, "routed/shared alignment");
     a.routed = routed; a.routed_rows = routed_rows; a.inverse = inverse; a.rw = route_weight; a.shared = shared; a.K = top_k;
-    const int64_t row = int64_t(hidden) * 4, all = int64_t(routed_rows) * hidden * 2, picks = int64_t(tokens) * top_k * 4;
-    if (norm_overlap(a, {{h, row, row, tokens}, {shared, row, row, tokens}, gate_span(a), {routed, all, all, routed_rows ? 1 : 0},
-                         {inverse, picks, picks, 1}, {route_weight, picks, picks, 1}}))
+    const int64_t row = int64_t(hidden) * 4, half = int64_t(hidden) * 2, picks = int64_t(tokens) * top_k * 4;
+    // the one row of one token is its own; of more any token may read any
+    const RowSpan experts{routed, half, half, routed_rows}, none{};
+    const bool own = tokens == 1 && routed_rows == 1;
+    if (norm_overlap(a, {{h, row, row, tokens}, {shared, row, row, tokens}, gate_span(a), own ? experts : none},
+                     {own ? none : experts, {inverse, picks, picks, 1}, {route_weight, picks, picks, 1}}))
         return fail(GRIM_ERR_ARG, "an output overlaps another argument");
     return status(block_norm_launch(S(stream), a));
 }

@@ -368,8 +368,9 @@ int grimoire_rmsnorm_residual(void* stream, float* h, const float* r0, const flo
  * h_out = h' (may be NULL, may be h), out = o in fp32, out_bf = o in bf16
  * (either may be NULL; without both, pre_weight may be NULL).  The norm
  * weights are bf16 [hidden].  hidden % 4 == 0, <= 32768; fp32 rows 16-byte,
- * bf16 rows 8-byte aligned.  An output may take the place of an input of its
- * own type and row distance; it overlaps nothing else.  Sums are fp32; up to
+ * bf16 rows 8-byte aligned.  An output may take the place of h, x, shared or a
+ * gate [tokens][hidden] of its own type and row distance; it overlaps nothing
+ * else.  Sums are fp32; up to
  * 256 rows they are spread over more threads, so the last bits of a row may
  * differ from those it has in a larger batch.
  *   grimoire_block_norm: f = x[t], fp32 or (x_bf16) bf16 rows x_stride

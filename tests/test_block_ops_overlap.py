@@ -1,0 +1,66 @@
+"""Outputs of the block operators that share memory with an argument which
+other rows' work reads are refused: one at the same address, with the same
+width, is no argument that an output may take the place of.  Host checks
+only: what is not refused would reach a launch."""
+import ctypes as C
+import os
+
+import pytest
+
+from grimoire_amd import _abi
+
+pytestmark = pytest.mark.skipif(os.path.exists("/dev/kfd"), reason="made-up device addresses: no GPU may see them")
+
+ARG = _abi.ERR_ARG
+M = 1 << 20   # arguments that lie apart
+
+
+def launched(status):
+    """Past every check: the launch found no GPU."""
+    return status > 0
+
+
+def norm(T=3, H=64, gate=None, gate_kind=0, gate_bf16=0, moe=False, K=2, rows=7, **kw):
+    a = dict(h=M, x=2 * M, h_out=3 * M, out=4 * M, out_bf=5 * M, routed=6 * M, inverse=7 * M, rw=8 * M, shared=9 * M,
+             post=10 * M, pre=11 * M, x_bf16=0)
+    a.update(kw)
+    p = _abi.BlockNormParams(post_weight=a["post"], pre_weight=a["pre"], weight_offset=1.0, eps=1e-6,
+                             residual_scale=1.0, block_scale=1.0, gate_kind=gate_kind)
+    if moe:
+        return _abi.lib().grimoire_moe_block_norm(None, C.byref(p), gate, gate_bf16, a["h"], a["routed"], rows,
+                                                  a["inverse"], a["rw"], a["shared"], a["h_out"], a["out"],
+                                                  a["out_bf"], T, K, H)
+    return _abi.lib().grimoire_block_norm(None, C.byref(p), gate, gate_bf16, a["h"], a["x"], a["x_bf16"], H,
+                                          a["h_out"], a["out"], a["out_bf"], T, H)
+
+
+CHANNEL, ROW, FULL = _abi.GATE_CHANNEL, _abi.GATE_ROW, _abi.GATE_FULL
+
+
+@pytest.mark.parametrize("kw", [
+    dict(gate=3 * M, gate_kind=CHANNEL), dict(gate=4 * M, gate_kind=CHANNEL),
+    dict(gate=5 * M, gate_kind=CHANNEL, gate_bf16=1), dict(gate=3 * M, gate_kind=ROW, T=64),
+    dict(gate=5 * M, gate_kind=ROW, gate_bf16=1, T=64), dict(gate=3 * M + 256, gate_kind=CHANNEL)])
+@pytest.mark.parametrize("moe", [False, True])
+def test_gate_of_many_rows(kw, moe):
+    assert norm(moe=moe, **kw) == ARG
+
+
+@pytest.mark.parametrize("kw", [
+    dict(T=16, K=4, rw=3 * M), dict(T=16, K=4, rw=4 * M), dict(T=16, K=4, inverse=3 * M),
+    dict(T=16, K=4, inverse=4 * M), dict(T=32, K=4, inverse=5 * M),          # T K = H (H / 2 beside the bf16 rows)
+    dict(rows=1, routed=5 * M), dict(rows=2, routed=3 * M), dict(rows=2, routed=4 * M), dict(T=1, rows=2, routed=3 * M),
+    dict(T=1, K=4, H=4, rw=3 * M)])
+def test_routes_and_expert_rows(kw):
+    assert norm(moe=True, **kw) == ARG
+
+
+@pytest.mark.parametrize("kw", [
+    dict(h_out=M), dict(out=M), dict(x=4 * M), dict(x=5 * M, x_bf16=1), dict(gate=4 * M, gate_kind=FULL),
+    dict(gate=5 * M, gate_kind=FULL, gate_bf16=1), dict(moe=True, shared=3 * M), dict(moe=True, h_out=M, shared=4 * M),
+    dict(T=1, gate=3 * M, gate_kind=CHANNEL), dict(moe=True, T=1, rows=1, routed=5 * M),
+    dict(gate=3 * M + 768, gate_kind=CHANNEL), dict()])
+def test_in_place_stays(kw):
+    """h, x, shared and a full gate of an output's own layout; what one row alone
+    reads."""
+    assert launched(norm(**kw))
