@@ -502,7 +502,7 @@ int grimoire_rmsnorm_residual(void* stream, float* h, const float* r0, const flo
 // An output of a block norm may take the place of one of the inputs `rows`, of
 // its own type, distance and number of rows (each row is read before it is
 // written, by the work-group that writes it), and overlaps nothing else: of
-// `whole` any row may read any part.
+// `whole` and the norm weights any row may read any part.
 static bool norm_overlap(const BlockNormArgs& a, std::initializer_list<RowSpan> rows,
                          std::initializer_list<RowSpan> whole) {
     const int64_t f = int64_t(a.H) * 4, b = int64_t(a.H) * 2;
@@ -512,6 +512,7 @@ static bool norm_overlap(const BlockNormArgs& a, std::initializer_list<RowSpan> 
             if (share_memory(outs[i], in) && !same_rows(outs[i], in)) return true;
         for (const RowSpan& in : whole)
             if (share_memory(outs[i], in)) return true;
+        if (share_memory(outs[i], {a.post_w, b, b, 1}) || share_memory(outs[i], {a.pre_w, b, b, 1})) return true;
         for (int j = 0; j < i; ++j)
             if (share_memory(outs[i], outs[j])) return true;
     }

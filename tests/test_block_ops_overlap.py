@@ -64,3 +64,12 @@ def test_in_place_stays(kw):
     """h, x, shared and a full gate of an output's own layout; what one row alone
     reads."""
     assert launched(norm(**kw))
+
+
+@pytest.mark.parametrize("kw", [dict(post=3 * M), dict(post=4 * M + 704), dict(pre=5 * M), dict(pre=3 * M - 64),
+                                dict(pre=4 * M + 8), dict(T=1, pre=5 * M), dict(T=1, post=5 * M)])
+@pytest.mark.parametrize("moe", [False, True])
+def test_norm_weights(kw, moe):
+    assert norm(moe=moe, **kw) == ARG
+    assert launched(norm(moe=moe, post=None)) and launched(norm(moe=moe, pre=None, out=None, out_bf=None))
+    assert launched(norm(moe=moe, post=11 * M, pre=3 * M + 768))
