@@ -339,8 +339,10 @@ int grimoire_moe_router_scores(void* stream, const grim_score_params* p, const v
     const int64_t size = logits_bf16 ? 2 : 4, picks = int64_t(top_k) * 4;
     const RowSpan in{logits, row_stride * size, n_experts * size, tokens};
     const RowSpan ids{out_expert, picks, picks, tokens}, weights{out_weight, picks, picks, tokens};
-    if (share_memory(in, ids) || share_memory(in, weights) || share_memory(ids, weights))
-        return fail(GRIM_ERR_ARG, "logits and outputs overlap");
+    const RowSpan bias{p->bias, n_experts * int64_t(4), n_experts * int64_t(4), 1};
+    if (share_memory(in, ids) || share_memory(in, weights) || share_memory(ids, weights) ||
+        share_memory(bias, ids) || share_memory(bias, weights))
+        return fail(GRIM_ERR_ARG, "an output overlaps another argument");
     ScoresArgs a{logits, row_stride, logits_bf16 ? 1 : 0, tokens, n_experts, top_k,
                  p->score == GRIM_SCORE_SIGMOID, p->bias, G, G > 1 ? p->topk_group : 1,
                  p->group_score == GRIM_GROUP_TOP2, p->normalize, p->scaling, out_expert, out_weight};

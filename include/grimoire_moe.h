@@ -181,8 +181,8 @@ int grimoire_moe_router_topk_group(void* stream, const float* logits, const floa
  * expert -1, weight 0 (the products skip such routes).  Scores, sums and the
  * choice are fp64, so the routing does not depend on fp32 rounding.
  * logits: fp32 or (logits_bf16) bf16 rows, row_stride elements apart
- * (>= n_experts), apart from both outputs.  n_experts <= 512, top_k <= min(16, n_experts), and with
- * groups <= topk_group * (n_experts / n_group). */
+ * (>= n_experts).  The outputs overlap nothing.  n_experts <= 512, top_k <=
+ * min(16, n_experts), and with groups <= topk_group * (n_experts / n_group). */
 enum grim_score {
     GRIM_SCORE_SOFTMAX = 0,
     GRIM_SCORE_SIGMOID = 1

@@ -73,3 +73,14 @@ def test_norm_weights(kw, moe):
     assert norm(moe=moe, **kw) == ARG
     assert launched(norm(moe=moe, post=None)) and launched(norm(moe=moe, pre=None, out=None, out_bf=None))
     assert launched(norm(moe=moe, post=11 * M, pre=3 * M + 768))
+
+
+def scores(bias=3 * M, E=64, K=8, T=2, logits=M, ids=2 * M, w=2 * M + 4096):
+    p = _abi.ScoreParams(score=0, n_group=1, topk_group=1, group_score=0, normalize=1, scaling=1.0, bias=bias)
+    return _abi.lib().grimoire_moe_router_scores(None, C.byref(p), logits, 0, E, T, E, K, ids, w)
+
+
+@pytest.mark.parametrize("kw", [dict(bias=2 * M), dict(bias=2 * M - 252), dict(bias=2 * M + 60), dict(bias=2 * M + 4096)])
+def test_scores_bias(kw):
+    assert scores(**kw) == ARG
+    assert launched(scores()) and launched(scores(bias=None)) and launched(scores(bias=2 * M + 64))
