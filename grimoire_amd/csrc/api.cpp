@@ -632,6 +632,12 @@ static int lora_common(void* stream, const grim_lora* L, const int32_t* row_slot
     const size_t need = lora_workspace_bytes(L->K, L->max_rank, rows);
     if (!ws || ws_bytes < need) return fail(GRIM_ERR_WORKSPACE, "adapter workspace too small (need %zu)", need);
     if (!aligned(ws, 16)) return fail(GRIM_ERR_ARG, "workspace not 16-byte aligned");
+    // what any work-group may read, whatever rows it writes
+    const int64_t slots = L->slots, ab = slots * L->max_rank * L->K * 2, bb = slots * L->max_rank * L->N * 2;
+    const RowSpan read[] = {{row_slot, rows * int64_t(4), rows * int64_t(4), 1}, {L->a, ab, ab, 1}, {L->b, bb, bb, 1},
+                            {L->rank, slots * 4, slots * 4, 1}, {L->scale, slots * 4, slots * 4, 1}};
+    for (const RowSpan& r : read)
+        if (share_memory(out, r)) return fail(GRIM_ERR_ARG, "the output overlaps the adapters or row_slot");
     LoraArgs a{};
     a.a = L->a; a.b = L->b; a.rank = L->rank; a.scale = L->scale;
     a.slots = L->slots; a.R = L->max_rank; a.K = L->K; a.N = L->N;

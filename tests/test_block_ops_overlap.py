@@ -84,3 +84,31 @@ def scores(bias=3 * M, E=64, K=8, T=2, logits=M, ids=2 * M, w=2 * M + 4096):
 def test_scores_bias(kw):
     assert scores(**kw) == ARG
     assert launched(scores()) and launched(scores(bias=None)) and launched(scores(bias=2 * M + 64))
+
+
+LORA = dict(x=M, base=2 * M, y=3 * M, slot=4 * M, a=5 * M, b=6 * M, rank=7 * M, scale=8 * M, ws=9 * M)
+LORA_BYTES = dict(slot=3 * 4, a=4 * 16 * 64 * 2, b=4 * 32 * 16 * 2, rank=4 * 4, scale=4 * 4)
+
+
+def lora(glu=False, rows=3, **kw):
+    a = dict(LORA, **kw)
+    L = _abi.Lora(K=64, N=32, slots=4, max_rank=16, a=a["a"], b=a["b"], rank=a["rank"], scale=a["scale"])
+    need = _abi.lib().grimoire_lora_workspace_bytes(C.byref(L), rows)
+    fn = _abi.lib().grimoire_lora_swiglu if glu else _abi.lib().grimoire_lora_add
+    return fn(None, C.byref(L), a["slot"], a["x"], 0, 64, a["base"], 0, 32, a["y"], 0, 16 if glu else 32, rows,
+              a["ws"], need)
+
+
+@pytest.mark.parametrize("name", list(LORA_BYTES))
+@pytest.mark.parametrize("glu", [False, True])
+def test_adapter_output(name, glu):
+    """An output over the adapters, their ranks and scales or the rows' slots."""
+    y, n = LORA["y"], 3 * (16 if glu else 32) * 4
+    last = LORA_BYTES[name]
+    for at in (y, y + n - 16, y - last // 16 * 16 + (16 if last % 16 == 0 else 0)):
+        assert lora(glu, **{name: at}) == ARG
+        # in place it is an output all the same
+        assert glu or lora(base=y, **{name: at}) == ARG
+    for at in (y + n, y - (last + 15) // 16 * 16):
+        assert launched(lora(glu, **{name: at}))
+    assert launched(lora(glu)) and (glu or launched(lora(base=y)))
