@@ -636,8 +636,14 @@ static int lora_common(void* stream, const grim_lora* L, const int32_t* row_slot
     const int64_t slots = L->slots, ab = slots * L->max_rank * L->K * 2, bb = slots * L->max_rank * L->N * 2;
     const RowSpan read[] = {{row_slot, rows * int64_t(4), rows * int64_t(4), 1}, {L->a, ab, ab, 1}, {L->b, bb, bb, 1},
                             {L->rank, slots * 4, slots * 4, 1}, {L->scale, slots * 4, slots * 4, 1}};
-    for (const RowSpan& r : read)
+    const RowSpan work{ws, int64_t(need), int64_t(need), 1};
+    for (const RowSpan& r : read) {
         if (share_memory(out, r)) return fail(GRIM_ERR_ARG, "the output overlaps the adapters or row_slot");
+        if (share_memory(work, r)) return fail(GRIM_ERR_ARG, "the workspace overlaps the adapters or row_slot");
+    }
+    if (share_memory(work, out) || share_memory(work, {x, x_stride * xz, L->K * xz, rows}) ||
+        share_memory(work, {base, base_stride * bz, L->N * bz, rows}))
+        return fail(GRIM_ERR_ARG, "the workspace overlaps x, base or the output");
     LoraArgs a{};
     a.a = L->a; a.b = L->b; a.rank = L->rank; a.scale = L->scale;
     a.slots = L->slots; a.R = L->max_rank; a.K = L->K; a.N = L->N;

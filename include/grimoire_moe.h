@@ -426,8 +426,9 @@ typedef struct grim_lora {
 } grim_lora;
 
 /* Device workspace of the calls below for up to `rows` rows (16-byte
- * aligned, no initial contents needed).  Calls that share one must not
- * overlap: two graphs that hold it run one after the other. */
+ * aligned, no initial contents needed, apart from every other argument).
+ * Calls that share one must not overlap: two graphs that hold it run one
+ * after the other. */
 size_t grimoire_lora_workspace_bytes(const grim_lora* L, int rows);
 /* y[t] = base[t] + scale_a B_a (A_a x[t]); rows without an adapter are
  * copied (in place: left as they are).  x [rows][K], base and y [rows][N]:

@@ -112,3 +112,19 @@ def test_adapter_output(name, glu):
     for at in (y + n, y - (last + 15) // 16 * 16):
         assert launched(lora(glu, **{name: at}))
     assert launched(lora(glu)) and (glu or launched(lora(base=y)))
+
+
+@pytest.mark.parametrize("name,n", [("x", 3 * 64 * 4), ("base", 3 * 32 * 4), ("y", 3 * 16 * 4), *LORA_BYTES.items()])
+@pytest.mark.parametrize("glu", [False, True])
+def test_adapter_workspace(name, n, glu):
+    """The workspace apart from everything: z is written while x, the slots,
+    the adapters and ranks are read, and read while y is written."""
+    L = _abi.Lora(K=64, N=32, slots=4, max_rank=16)
+    need = int(_abi.lib().grimoire_lora_workspace_bytes(C.byref(L), 3))
+    at, n = LORA[name], (n + 15) // 16 * 16
+    for ws in (at, at + n - 16, at - need + 16):
+        assert lora(glu, ws=ws) == ARG
+    if name != "y" or glu:
+        for ws in (at + n, at - need):
+            assert launched(lora(glu, ws=ws))
+    assert glu or lora(base=LORA["y"], ws=LORA["y"]) == ARG
