@@ -579,9 +579,10 @@ int grimoire_moe_block_norm(void* stream, const grim_block_norm_params* p, const
     if (tokens <= 0) return GRIM_OK;
     BlockNormArgs a;
     if (int r = block_norm_args(p, gate, gate_bf16, h, h_out, out, out_bf, tokens, hidden, a)) return r;
-    if (!routed || !inverse || !route_weight) return fail(GRIM_ERR_ARG, "null routed/inverse/weights");
-    if (top_k <= 0 || top_k > 16) return fail(GRIM_ERR_SHAPE, "top_k=%d (1..16)", top_k);
     if (routed_rows < 0) return fail(GRIM_ERR_SHAPE, "routed_rows=%d", routed_rows);
+    if ((!routed && routed_rows) || !inverse || !route_weight)
+        return fail(GRIM_ERR_ARG, "null routed/inverse/weights");
+    if (top_k <= 0 || top_k > 16) return fail(GRIM_ERR_SHAPE, "top_k=%d (1..16)", top_k);
     if (!aligned(routed, 8) || !aligned(shared, 16)) return fail(GRIM_ERR_ARG, "routed/shared alignment");
     a.routed = routed; a.routed_rows = routed_rows; a.inverse = inverse; a.rw = route_weight; a.shared = shared; a.K = top_k;
     const int64_t row = int64_t(hidden) * 4, half = int64_t(hidden) * 2, picks = int64_t(tokens) * top_k * 4;

@@ -377,7 +377,7 @@ int grimoire_rmsnorm_residual(void* stream, float* h, const float* r0, const flo
  *     elements apart (a multiple of 4, >= hidden).
  *   grimoire_moe_block_norm: f = shared[t] (fp32, may be NULL) + sum_s
  *     route_weight[t,s] * routed[inverse[t,s]], an fma chain in slot order;
- *     routed bf16 [routed_rows][hidden];
+ *     routed bf16 [routed_rows][hidden] (NULL where there are none);
  *     a slot whose inverse lies outside [0, routed_rows) is skipped;
  *     top_k <= 16: the combine of grimoire_moe_rmsnorm_residual. */
 enum grim_gate_kind {
