@@ -956,7 +956,7 @@ static int forward_impl(void* stream, const grim_moe_layer* L, const grim_route_
     {
         ScoresArgs sa{p.logits, E, 0, tokens, E, K, 0, probs ? static_cast<const float*>(rp->bias) : nullptr,
                       probs && rp->n_group > 1 ? rp->n_group : 1, probs ? rp->topk_group : 1, 0, c.norm_topk,
-                      scaling, p.rex, p.rwt, tka.part1, nullptr};
+                      scaling, p.rex, p.rwt, tka.part1};
         hipError_t e = probs ? scores_launch(st, sa) : topk_launch(st, tka);
         if (e != hipSuccess) return ferr(int(e), hipGetErrorString(e));
     }

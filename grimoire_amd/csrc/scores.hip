@@ -138,10 +138,6 @@ __global__ __launch_bounds__(kScWaves * kWave) void scores_kernel(ScoresArgs a, 
     if (a.part1) {
 #pragma unroll
         for (int j = 0; j < NV; ++j) lv[j] += a.part1[row + at[j]];
-        if (a.lbias) {
-#pragma unroll
-            for (int j = 0; j < NV; ++j) lv[j] += a.lbias[at[j]];
-        }
     }
     // an expert that is out (NaN too, which fmaxf drops): -inf; +inf is the
     // largest finite logit

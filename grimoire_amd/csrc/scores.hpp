@@ -18,10 +18,9 @@ struct ScoresArgs {
     float scaling;
     int32_t* out_e;           // [T][K]
     float* out_w;
-    // split-K router partials (fp32 logits): the row is (logits + part1) +
-    // lbias, both with the logits' layout / [E]
+    // the split-K router's second partial sum (fp32 logits), laid out as the
+    // logits: the row is logits + part1
     const float* part1 = nullptr;
-    const float* lbias = nullptr;
 };
 
 constexpr int kScoresMaxE = 512, kScoresMaxK = 16, kScoresMaxGroups = 64;
