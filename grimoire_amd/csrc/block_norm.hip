@@ -12,7 +12,12 @@
 //
 // 4096 x 7168, bf16 block output, bf16 gate an element: 98.6 us, 5.4 TB/s
 // (a large copy: 4.94); 3001 x 2048 behind ten experts and a shared one: 48.2
-// us, 4.9 TB/s.  One to 32 rows: 3 to 7 us, two barriers and a chain of loads.
+// us, 4.9 TB/s.  One to 32 rows: 4 to 8 us, two barriers and a chain of loads.
+// Above 8192 columns a row takes 1024 threads of 92 registers and more, one
+// work-group a CU: 2048 x 16384, bf16 block output 96 us, 4.2 TB/s.  Above
+// 16384 a thread's eight chunks leave no registers for the norm weights ahead,
+// and 2 to 8 are spilled (24 with 16 routes): 1024 x 32768 112 us, 3.6 TB/s;
+// 512 x 32768 behind ten experts 122 us, 4.1 TB/s.
 #include "block_norm.hpp"
 
 namespace grim {
@@ -32,8 +37,9 @@ __device__ __forceinline__ F4 widen(uint2 u) {
 }
 __device__ __forceinline__ F4 load_b16(const uint16_t* p) { return widen(*reinterpret_cast<const uint2*>(p)); }
 
-// 1 / (1 + exp(-g)) by the hardware exp2 and reciprocal (about 1 ulp each):
-// the gate scales an fp32 sum that is compared to a tolerance.
+// 1 / (1 + exp(-g)) by the hardware exp2 and reciprocal (about 1 ulp each,
+// plus the rounding of the exponent, up to |g| 2^-23 relative): the gate scales
+// an fp32 sum that is compared to a tolerance.
 __device__ __forceinline__ float gate_act(float g, int sigmoid) {
     return sigmoid ? __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(g * -1.44269504088896341f)) : g;
 }

@@ -16,8 +16,13 @@
 // TB/s of a large copy): 4096 rows of 9 requests, 2048 -> 7168, rank 64 of
 // mixed ranks, bf16: 13 + 37 (28; base copied to y by the same loop 25.5);
 // 2001 rows of 5, 2880 -> 2 x 2880, rank 16, fp32: 11 + 19 (19); 48 mixed
-// rows of 32 adapters, 2048 -> 7168: 5 + 11 (3.3); one row, 768 -> 2048: 5 in
+// rows of 32 adapters, 2048 -> 7168: 5 + 10 (3.3); one row, 768 -> 2048: 5 in
 // one launch, a chain of dependent loads.
+//
+// Long batches should hold their rows in runs of one adapter: rows are tiled
+// in the order they come in, and a tile reads A and B once for every adapter
+// it names.  2048 -> 7168, 32 adapters of rank 64, bf16, both launches: 4096
+// rows in 9 runs 52 us, in no order 367; 1024 in no order 117, 512 63, 256 40.
 //
 // fp32 values are multiplied exactly: an fp32 x (and z) is the sum of three
 // bf16 pieces of 8 significant bits, cut off, not rounded, so each rest is
@@ -701,7 +706,8 @@ void shrink(hipStream_t st, const LoraArgs& a, int splits, int items) {
 // every tile is one adapter's, which leaves room for the tiles of two (4096
 // rows of 9 requests, 2048 -> 7168: 34.8 us; runs that fill the chip: 40.4);
 // three of them share out tiles of many (48 mixed rows of 32 adapters:
-// 15.4 us in all; with two or four 18.4, 17.0).
+// 15.4 us in all; with two or four 18.4, 17.0).  Measured at rank 64 alone;
+// above 64 a CU holds two or three work-groups.
 constexpr int kExpandRuns = 512, kExpandGroups = 768;
 
 template <bool GLU, bool BB>

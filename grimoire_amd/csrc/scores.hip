@@ -8,9 +8,13 @@
 // slots nothing is left for get expert -1 and weight 0.
 //
 // The scores are formed in fp64.  A choice is a border: in fp32 two scores
-// closer than their rounding (an exp and a sum over E) swap places with the
-// order of the sum, about once in 10^5 picks at E = 512; in fp64 the choice
-// is that of the exact scores.  It costs E exps of the fp64 pipe a token.
+// closer than their rounding (an exp, a sum over E, a bias) swap places with
+// the order of the sum (Gaussian logits, a balance bias of 0.3 / E: 3 of
+// 4.9 million picks at E = 512, 6 of 3.9 million at E = 256), and scores that
+// saturate are equal (sigmoids of logits above 18 all round to 1); in fp64 the
+// choice is that of the exact scores.  It costs E exps of the fp64 pipe a
+// token, also where no bias and no sum of two makes the order another than the
+// logits' own.
 //
 // Lanes: without groups expert e is lane e % 64's, so a load of a lane's j-th
 // expert is one run of memory.  With groups each owns lpg =
@@ -22,9 +26,9 @@
 // experts that reach it are gathered, one a lane, and ranked against each
 // other in fp64.  More than 64 of them (ties) take K rounds over all values.
 //
-// 4096 tokens, 512 experts, top 10, bias: 8.2 us (the logits' bytes take 1.8
-// at the rate of a large copy): vector issue bounds it, 726 instructions a
-// token, 210 of them the exps (K rounds of wave maxima in place of the search
+// 4096 tokens, 512 experts, top 10, bias: 8.1 us (the logits' bytes take 1.8
+// at the rate of a large copy): vector issue bounds this form of it, 726
+// instructions a token, 210 of them the exps (K rounds of wave maxima in place of the search
 // and the ranking: 925 and 10.2 us; over the fp64 values: 16.0).  One token
 // of 128 experts: 3 us.
 #include "scores.hpp"

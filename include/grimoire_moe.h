@@ -179,7 +179,9 @@ int grimoire_moe_router_topk_group(void* stream, const float* logits, const floa
  * An expert is out when its logit is NaN or -inf or its s' is NaN or -inf;
  * +inf counts as the largest finite logit.  Slots no expert is left for get
  * expert -1, weight 0 (the products skip such routes).  Scores, sums and the
- * choice are fp64, so the routing does not depend on fp32 rounding.
+ * choice are fp64, so the routing does not depend on fp32 rounding; the
+ * sigmoid with groups of grimoire_moe_router_topk_group is fp32, and the two
+ * may choose differently between scores that fp32 does not tell apart.
  * logits: fp32 or (logits_bf16) bf16 rows, row_stride elements apart
  * (>= n_experts).  The outputs overlap nothing.  n_experts <= 512, top_k <=
  * min(16, n_experts), and with groups <= topk_group * (n_experts / n_group). */
@@ -370,9 +372,9 @@ int grimoire_rmsnorm_residual(void* stream, float* h, const float* r0, const flo
  * weights are bf16 [hidden].  hidden % 4 == 0, <= 32768; fp32 rows 16-byte,
  * bf16 rows 8-byte aligned.  An output may take the place of h, x, shared or a
  * gate [tokens][hidden] of its own type and row distance; it overlaps nothing
- * else.  Sums are fp32; up to
- * 256 rows they are spread over more threads, so the last bits of a row may
- * differ from those it has in a larger batch.
+ * else.  Sums are fp32; up to 256 rows they are spread over more threads, so
+ * the last bits of a row may differ from those it has in a larger batch.
+ * Rows up to 8192 run at the rate of a copy, longer ones below it.
  *   grimoire_block_norm: f = x[t], fp32 or (x_bf16) bf16 rows x_stride
  *     elements apart (a multiple of 4, >= hidden).
  *   grimoire_moe_block_norm: f = shared[t] (fp32, may be NULL) + sum_s
@@ -439,7 +441,8 @@ size_t grimoire_lora_workspace_bytes(const grim_lora* L, int rows);
  * beside each other in one buffer.  Sums are fp32, in an order that does not
  * depend on the other rows' adapters; fp32 activations are multiplied in full
  * precision.  An adapter weight that is not finite makes NaN or infinity of
- * what it is multiplied into, in its own adapter's rows only. */
+ * what it is multiplied into, in its own adapter's rows only.  Batches above
+ * a few hundred rows are fastest with each adapter's rows side by side. */
 int grimoire_lora_add(void* stream, const grim_lora* L, const int32_t* row_slot, const void* x, int x_bf16,
                       int64_t x_stride, const void* base, int base_bf16, int64_t base_stride, void* y,
                       int y_bf16, int64_t y_stride, int rows, void* workspace, size_t workspace_bytes);
@@ -864,7 +867,8 @@ size_t grimoire_moe_forward_workspace_bytes(const grim_moe_layer* L, int tokens)
  * GEMV (MXFP4 with hidden and inter multiples of 64 above 256: on the
  * scaled fp4 matrix core, K padded to 256; otherwise on the vector ALU), 5 = expert-grouped GEMV on
  * the vector ALU.  GRIM_ROUTE_PROBS routes in a launch of its own: regimes 1
- * and 7 run as 3.  No reference counterpart for 3-5 (regimes of this
+ * and 7 run as 3, and regime 0 takes neither the decode kernels nor a top-k
+ * inside the dispatch.  No reference counterpart for 3-5 (regimes of this
  * build; the reference picks its kernels per batch size the same way). */
 int grimoire_moe_forward(void* stream, const grim_moe_layer* L, const grim_route_params* rp,
                          const uint16_t* shared_gate_w, const float* x, float* y, int tokens,
