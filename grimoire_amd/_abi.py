@@ -164,6 +164,7 @@ SIGNATURES = {
     "grimoire_moe_router_topk_sigmoid": (I32, [P, P, P, I32, I32, I32, P, P, I32, F32]),
     "grimoire_moe_router_topk_group": (I32, [P, P, P, I32, I32, I32, I32, I32, P, P, I32, F32]),
     "grimoire_moe_router_scores": (I32, [P, C.POINTER(ScoreParams), P, I32, I64, I32, I32, I32, P, P]),
+    "grimoire_moe_router_scores_grad": (I32, [P, C.POINTER(ScoreParams), P, I32, I64, P, P, P, I64, I32, I32, I32]),
     "grimoire_moe_gate_up": (I32, [P, LP, P, P, P]),
     "grimoire_moe_down": (I32, [P, LP, P, P, P, P]),
     "grimoire_moe_gate_up_shared": (I32, [P, LP, QWP, P, P, P, P, P]),
@@ -189,6 +190,12 @@ SIGNATURES = {
     "grimoire_block_norm": (I32, [P, C.POINTER(BlockNormParams), P, I32, P, P, I32, I64, P, P, P, I32, I32]),
     "grimoire_moe_block_norm": (I32, [P, C.POINTER(BlockNormParams), P, I32, P, P, I32, P, P, P, P, P, P, I32,
                                       I32, I32]),
+    "grimoire_moe_sort_rows": (I32, [P, P, P, I32, I64, P, P, I32, P, P, P, P, I32, I32, I32, I32, P, SZ]),
+    "grimoire_moe_sort_rows_grad": (I32, [P, P, I32, I64, P, P, P, I32, I64, P, I32, I64, P, I32, I32, I32]),
+    "grimoire_moe_combine_grad": (I32, [P, P, I32, I64, P, I32, I64, P, P, P, P, P, I32, P, P, P, I32, I32, I32]),
+    "grimoire_proj4_workspace_bytes": (SZ, [QWP, I32]),
+    "grimoire_proj4": (I32, [P, QWP, P, I32, I64, P, I32, I64, P, I32, I64, I32, P, SZ]),
+    "grimoire_proj4_swiglu": (I32, [P, QWP, P, I32, I64, P, I32, I64, I32, P, SZ]),
     "grimoire_lora_workspace_bytes": (SZ, [C.POINTER(Lora), I32]),
     "grimoire_lora_add": (I32, [P, C.POINTER(Lora), P, P, I32, I64, P, I32, I64, P, I32, I64, I32, P, SZ]),
     "grimoire_lora_swiglu": (I32, [P, C.POINTER(Lora), P, P, I32, I64, P, I32, I64, P, I32, I64, I32, P, SZ]),

@@ -22,9 +22,12 @@
 #include "elementwise.hpp"
 #include "ingest.hpp"
 #include "lora.hpp"
+#include "proj4.hpp"
 #include "tiered.hpp"
 #include "router.hpp"
 #include "scores.hpp"
+#include "scores_grad.hpp"
+#include "sort_rows.hpp"
 #include "gemv_mx.hpp"
 
 using namespace grim;
@@ -313,6 +316,29 @@ static bool same_rows(const RowSpan& a, const RowSpan& b) {
     return a.p == b.p && a.stride == b.stride && a.width == b.width && a.rows == b.rows;
 }
 
+static bool aligned(const void* p, uintptr_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+
+// Rows of a call below: fp32 or bf16, `stride` elements apart.
+static bool rows_aligned(const void* p, int b16) { return aligned(p, b16 ? 8 : 16); }
+static RowSpan row_span(const void* p, int b16, int64_t stride, int64_t width, int64_t rows) {
+    const int64_t size = b16 ? 2 : 4;
+    return {p, stride * size, width * size, rows};
+}
+static RowSpan whole(const void* p, int64_t bytes) { return {p, bytes, bytes, 1}; }
+static bool any_shared(std::initializer_list<RowSpan> outs, std::initializer_list<RowSpan> ins) {
+    for (const RowSpan* o = outs.begin(); o != outs.end(); ++o) {
+        for (const RowSpan& i : ins)
+            if (share_memory(*o, i)) return true;
+        for (const RowSpan* p = outs.begin(); p != o; ++p)
+            if (share_memory(*o, *p)) return true;
+    }
+    return false;
+}
+constexpr int64_t kMaxRowStride = int64_t(1) << 28;     // elements: 2^31 rows stay within 64 bits of bytes
+static bool stride_ok(int64_t stride, int hidden, int multiple) {
+    return stride >= hidden && stride <= kMaxRowStride && stride % multiple == 0;
+}
+
 int grimoire_moe_router_scores(void* stream, const grim_score_params* p, const void* logits,
                                int logits_bf16, int64_t row_stride, int tokens, int n_experts,
                                int top_k, int32_t* out_expert, float* out_weight) {
@@ -347,6 +373,32 @@ int grimoire_moe_router_scores(void* stream, const grim_score_params* p, const v
                  p->score == GRIM_SCORE_SIGMOID, p->bias, G, G > 1 ? p->topk_group : 1,
                  p->group_score == GRIM_GROUP_TOP2, p->normalize, p->scaling, out_expert, out_weight};
     return status(scores_launch(S(stream), a));
+}
+
+int grimoire_moe_router_scores_grad(void* stream, const grim_score_params* p, const void* logits,
+                                    int logits_bf16, int64_t row_stride, const int32_t* expert,
+                                    const float* dweight, void* dlogits, int64_t d_stride, int tokens,
+                                    int n_experts, int top_k) {
+    if (tokens <= 0) return GRIM_OK;
+    if (!p || !logits || !expert || !dweight || !dlogits) return fail(GRIM_ERR_ARG, "null pointer");
+    if (p->score != GRIM_SCORE_SOFTMAX && p->score != GRIM_SCORE_SIGMOID)
+        return fail(GRIM_ERR_ARG, "score=%d", p->score);
+    if (n_experts <= 0 || n_experts > kScoresMaxE)
+        return fail(GRIM_ERR_SHAPE, "n_experts=%d (1..%d)", n_experts, kScoresMaxE);
+    if (top_k <= 0 || top_k > kScoresMaxK || top_k > n_experts)
+        return fail(GRIM_ERR_SHAPE, "top_k=%d (1..%d)", top_k, kScoresMaxK);
+    if (!stride_ok(row_stride, n_experts, 1) || !stride_ok(d_stride, n_experts, 1))
+        return fail(GRIM_ERR_SHAPE, "row_stride=%lld d_stride=%lld", (long long)row_stride,
+                    (long long)d_stride);
+    const int64_t size = logits_bf16 ? 2 : 4, picks = int64_t(top_k) * 4;
+    const RowSpan in{logits, row_stride * size, n_experts * size, tokens};
+    const RowSpan out{dlogits, d_stride * size, n_experts * size, tokens};
+    if ((share_memory(out, in) && !same_rows(out, in)) || share_memory(out, {expert, picks, picks, tokens}) ||
+        share_memory(out, {dweight, picks, picks, tokens}))
+        return fail(GRIM_ERR_ARG, "dlogits overlaps another argument");
+    ScoresGradArgs a{logits, expert, dweight, dlogits, row_stride, d_stride, logits_bf16 ? 1 : 0, tokens,
+                     n_experts, top_k, p->score == GRIM_SCORE_SIGMOID, p->normalize ? 1 : 0, p->scaling};
+    return status(scores_grad_launch(S(stream), a));
 }
 
 int grimoire_moe_gate_up(void* stream, const grim_moe_layer* L, const int32_t* d_expert,
@@ -527,8 +579,6 @@ static RowSpan gate_span(const BlockNormArgs& a) {
     return {a.gate, n, n, 1};
 }
 
-static bool aligned(const void* p, uintptr_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
-
 // What both forms of the block norm check and share.
 static int block_norm_args(const grim_block_norm_params* p, const void* gate, int gate_bf16, const float* h,
                            float* h_out, float* out, uint16_t* out_bf, int tokens, int hidden,
@@ -593,6 +643,147 @@ int grimoire_moe_block_norm(void* stream, const grim_block_norm_params* p, const
                      {own ? none : experts, {inverse, picks, picks, 1}, {route_weight, picks, picks, 1}}))
         return fail(GRIM_ERR_ARG, "an output overlaps another argument");
     return status(block_norm_launch(S(stream), a));
+}
+
+static int route_shape(int tokens, int top_k, int hidden) {
+    if (top_k <= 0 || top_k > 16) return fail(GRIM_ERR_SHAPE, "top_k=%d (1..16)", top_k);
+    if (hidden <= 0 || hidden % 4) return fail(GRIM_ERR_SHAPE, "hidden=%d (need %% 4)", hidden);
+    if (int64_t(tokens) * top_k > 0x7FFFFFFF) return fail(GRIM_ERR_SHAPE, "tokens * top_k above 2^31 - 1");
+    return GRIM_OK;
+}
+
+int grimoire_moe_sort_rows(void* stream, const int32_t* ids, const void* x, int x_bf16, int64_t x_stride,
+                           const float* weight, void* rows, int rows_bf16, int32_t* counts,
+                           int32_t* offsets, int32_t* inverse, int32_t* perm_token, int tokens,
+                           int hidden, int num_experts, int top_k, void* workspace,
+                           size_t workspace_bytes) {
+    if (tokens < 0) return GRIM_OK;
+    if (!counts || !offsets) return fail(GRIM_ERR_ARG, "null counts/offsets");
+    if (num_experts <= 0 || num_experts > kSortMaxE)
+        return fail(GRIM_ERR_SHAPE, "num_experts=%d (1..%d)", num_experts, kSortMaxE);
+    const int64_t eb = int64_t(num_experts) * 4, n = int64_t(tokens) * top_k;
+    SortRowsArgs a{ids, x, x_stride, weight, rows, counts, offsets, inverse, perm_token, x_bf16 ? 1 : 0,
+                   rows_bf16 ? 1 : 0, tokens, top_k, num_experts, hidden, workspace};
+    if (tokens == 0) {
+        if (any_shared({whole(counts, eb), whole(offsets, eb)}, {})) return fail(GRIM_ERR_ARG, "counts overlaps offsets");
+        return status(sort_rows_launch(S(stream), a));
+    }
+    if (!ids || !x || !rows || !inverse) return fail(GRIM_ERR_ARG, "null pointer");
+    if (int r = route_shape(tokens, top_k, hidden)) return r;
+    if (!stride_ok(x_stride, hidden, 4)) return fail(GRIM_ERR_SHAPE, "x_stride=%lld", (long long)x_stride);
+    if (!rows_aligned(x, x_bf16) || !rows_aligned(rows, rows_bf16))
+        return fail(GRIM_ERR_ARG, "fp32 rows 16-byte, bf16 rows 8-byte alignment");
+    const size_t need = dispatch_workspace_bytes(tokens, top_k, num_experts);
+    if (!workspace || workspace_bytes < need)
+        return fail(GRIM_ERR_WORKSPACE, "dispatch workspace too small (need %zu)", need);
+    if (!aligned(workspace, 4)) return fail(GRIM_ERR_ARG, "workspace alignment");
+    if (any_shared({row_span(rows, rows_bf16, hidden, hidden, n), whole(counts, eb), whole(offsets, eb),
+                    whole(inverse, n * 4), whole(perm_token, n * 4), whole(workspace, int64_t(need))},
+                   {row_span(x, x_bf16, x_stride, hidden, tokens), whole(ids, n * 4), whole(weight, n * 4)}))
+        return fail(GRIM_ERR_ARG, "an output overlaps another argument");
+    return status(sort_rows_launch(S(stream), a));
+}
+
+int grimoire_moe_sort_rows_grad(void* stream, const void* drows, int rows_bf16, int64_t n_rows,
+                                const int32_t* inverse, const float* weight, const void* x, int x_bf16,
+                                int64_t x_stride, void* dx, int dx_bf16, int64_t dx_stride,
+                                float* dweight, int tokens, int top_k, int hidden) {
+    if (tokens <= 0) return GRIM_OK;
+    if (!inverse || !dx || (!drows && n_rows > 0)) return fail(GRIM_ERR_ARG, "null pointer");
+    if (!weight != !x || !weight != !dweight) return fail(GRIM_ERR_ARG, "weight, x and dweight go together");
+    if (int r = route_shape(tokens, top_k, hidden)) return r;
+    if (n_rows < 0 || n_rows > 0x7FFFFFFF) return fail(GRIM_ERR_SHAPE, "n_rows=%lld", (long long)n_rows);
+    if (!stride_ok(dx_stride, hidden, 4) || (x && !stride_ok(x_stride, hidden, 4)))
+        return fail(GRIM_ERR_SHAPE, "x_stride=%lld dx_stride=%lld", (long long)x_stride, (long long)dx_stride);
+    if (!rows_aligned(drows, rows_bf16) || !rows_aligned(dx, dx_bf16) || !rows_aligned(x, x_bf16))
+        return fail(GRIM_ERR_ARG, "fp32 rows 16-byte, bf16 rows 8-byte alignment");
+    const int64_t n = int64_t(tokens) * top_k * 4;
+    if (any_shared({row_span(dx, dx_bf16, dx_stride, hidden, tokens), whole(dweight, n)},
+                   {row_span(drows, rows_bf16, hidden, hidden, n_rows), whole(inverse, n), whole(weight, n),
+                    row_span(x, x_bf16, x_stride, hidden, tokens)}))
+        return fail(GRIM_ERR_ARG, "an output overlaps another argument");
+    SortGradArgs a{drows, n_rows, inverse, weight, x, dx, dweight, x_stride, dx_stride, rows_bf16 ? 1 : 0,
+                   x_bf16 ? 1 : 0, dx_bf16 ? 1 : 0, tokens, top_k, hidden};
+    return status(sort_grad_launch(S(stream), a));
+}
+
+int grimoire_moe_combine_grad(void* stream, const void* dy, int dy_bf16, int64_t dy_stride,
+                              const void* rows, int rows_bf16, int64_t n_rows, const int32_t* inverse,
+                              const float* weight, void* drows, float* dweight, const void* shared,
+                              int shared_bf16, const float* gate, void* dshared, float* dgate,
+                              int tokens, int top_k, int hidden) {
+    if (tokens <= 0) return GRIM_OK;
+    if (!dy || !inverse || !weight || !dweight || ((!rows || !drows) && n_rows > 0))
+        return fail(GRIM_ERR_ARG, "null pointer");
+    if (!shared != !dshared || !gate != !dgate || (gate && !shared))
+        return fail(GRIM_ERR_ARG, "dshared goes with shared, dgate with gate, gate with shared");
+    if (int r = route_shape(tokens, top_k, hidden)) return r;
+    if (n_rows < 0 || n_rows > 0x7FFFFFFF) return fail(GRIM_ERR_SHAPE, "n_rows=%lld", (long long)n_rows);
+    if (!stride_ok(dy_stride, hidden, 4)) return fail(GRIM_ERR_SHAPE, "dy_stride=%lld", (long long)dy_stride);
+    if (!rows_aligned(dy, dy_bf16) || !rows_aligned(rows, rows_bf16) || !rows_aligned(drows, rows_bf16) ||
+        !rows_aligned(shared, shared_bf16) || !rows_aligned(dshared, shared_bf16))
+        return fail(GRIM_ERR_ARG, "fp32 rows 16-byte, bf16 rows 8-byte alignment");
+    const int64_t n = int64_t(tokens) * top_k * 4, tb = int64_t(tokens) * 4;
+    if (any_shared({row_span(drows, rows_bf16, hidden, hidden, n_rows), whole(dweight, n),
+                    row_span(dshared, shared_bf16, hidden, hidden, tokens), whole(dgate, tb)},
+                   {row_span(dy, dy_bf16, dy_stride, hidden, tokens), row_span(rows, rows_bf16, hidden, hidden, n_rows),
+                    whole(inverse, n), whole(weight, n), row_span(shared, shared_bf16, hidden, hidden, tokens),
+                    whole(gate, tb)}))
+        return fail(GRIM_ERR_ARG, "an output overlaps another argument");
+    CombineGradArgs a{dy, dy_stride, n_rows, rows, inverse, weight, drows, dweight, shared, gate, dshared, dgate,
+                      dy_bf16 ? 1 : 0, rows_bf16 ? 1 : 0, shared_bf16 ? 1 : 0, tokens, top_k, hidden};
+    return status(combine_grad_launch(S(stream), a));
+}
+
+size_t grimoire_proj4_workspace_bytes(const grim_quant_weight* w, int rows) {
+    (void)w;
+    (void)rows;
+    return 0;
+}
+
+static int proj4_common(void* stream, const grim_quant_weight* w, const void* x, int x_bf16, int64_t x_stride,
+                        const void* base, int base_bf16, int64_t base_stride, void* y, int y_bf16,
+                        int64_t y_stride, int rows, int glu) {
+    if (rows <= 0) return GRIM_OK;
+    if (!w || !x || !y) return fail(GRIM_ERR_ARG, "null pointer");
+    if (w->fmt != GRIM_FMT_INT4 && w->fmt != GRIM_FMT_INT4_F16 && w->fmt != GRIM_FMT_MXFP4)
+        return fail(GRIM_ERR_FORMAT, "projection: format %d (INT4, INT4_F16 or MXFP4)", w->fmt);
+    if (w->K <= 0 || w->N <= 0 || (glu && w->N % 2)) return fail(GRIM_ERR_SHAPE, "N=%d K=%d", w->N, w->K);
+    if (int r = check_weight(w, "projection", w->N, w->K)) return r;
+    if (w->fmt != GRIM_FMT_MXFP4 && !aligned(w->scales, 2)) return fail(GRIM_ERR_ARG, "scales alignment");
+    const int width = glu ? w->N / 2 : w->N;
+    if (!stride_ok(x_stride, w->K, 8)) return fail(GRIM_ERR_SHAPE, "x_stride=%lld", (long long)x_stride);
+    if (!stride_ok(y_stride, width, 1)) return fail(GRIM_ERR_SHAPE, "y_stride=%lld", (long long)y_stride);
+    if (base && !stride_ok(base_stride, width, 1))
+        return fail(GRIM_ERR_SHAPE, "base_stride=%lld", (long long)base_stride);
+    if (!aligned(x, 16) || !aligned(y, y_bf16 ? 2 : 4) || !aligned(base, base_bf16 ? 2 : 4))
+        return fail(GRIM_ERR_ARG, "x 16-byte, y and base an element's alignment");
+    const RowSpan out = row_span(y, y_bf16, y_stride, width, rows);
+    const RowSpan add = row_span(base, base_bf16, base_stride, width, rows);
+    const int64_t sb = int64_t(w->N) * w->row_scales;
+    if (any_shared({out}, {row_span(x, x_bf16, x_stride, w->K, rows), whole(w->payload, w->N * w->row_bytes),
+                           whole(w->scales, w->fmt == GRIM_FMT_MXFP4 ? sb : 2 * sb), whole(w->zeros, sb)}) ||
+        (share_memory(out, add) && (!same_rows(out, add) || !base_bf16 != !y_bf16)))
+        return fail(GRIM_ERR_ARG, "the output overlaps another argument");
+    Proj4Args a{view(*w), w->fmt, w->N, w->K, x, base, y, x_stride, base_stride, y_stride, x_bf16 ? 1 : 0,
+                base_bf16 ? 1 : 0, y_bf16 ? 1 : 0, rows, glu};
+    return status(proj4_launch(S(stream), a));
+}
+
+int grimoire_proj4(void* stream, const grim_quant_weight* w, const void* x, int x_bf16, int64_t x_stride,
+                   const void* base, int base_bf16, int64_t base_stride, void* y, int y_bf16,
+                   int64_t y_stride, int rows, void* workspace, size_t workspace_bytes) {
+    (void)workspace;
+    (void)workspace_bytes;
+    return proj4_common(stream, w, x, x_bf16, x_stride, base, base_bf16, base_stride, y, y_bf16, y_stride, rows, 0);
+}
+
+int grimoire_proj4_swiglu(void* stream, const grim_quant_weight* w, const void* x, int x_bf16,
+                          int64_t x_stride, void* h, int h_bf16, int64_t h_stride, int rows,
+                          void* workspace, size_t workspace_bytes) {
+    (void)workspace;
+    (void)workspace_bytes;
+    return proj4_common(stream, w, x, x_bf16, x_stride, nullptr, 0, 0, h, h_bf16, h_stride, rows, 1);
 }
 
 size_t grimoire_lora_workspace_bytes(const grim_lora* L, int rows) {

@@ -334,6 +334,11 @@ def _flat(t: Optional[torch.Tensor], what: str, shape, dtypes, dev: int):
     return t.data_ptr()
 
 
+def _routes(t: torch.Tensor, what: str, T: int, K: int, dev: int):
+    """Pointer of one int32 a route, [T*K] or [T][K]."""
+    return _flat(t, what, (T * K,) if t.dim() == 1 else (T, K), _I32, dev)
+
+
 def _gpu(t: torch.Tensor) -> int:
     dev = t.get_device()
     if dev < 0:
@@ -400,6 +405,24 @@ class RouteScores:
             raise _abi.GrimoireError("bias: one value an expert, on the logits' device")
         _launch(dev, stream, self._call, "router_scores", self._ref, lp, b16, stride, T, E, K,
                 _flat(out_expert, "out_expert", shape, _I32, dev), _flat(out_weight, "out_weight", shape, _F32, dev))
+
+    def grad(self, logits, expert, dweight, dlogits, stream=None):
+        """The gradient of the weights to the logits
+        (grimoire_moe_router_scores_grad): expert int32 [T][K] as chosen,
+        dweight fp32 [T][K], dlogits [T][E] of the logits' type (it may be the
+        logits).  Bias and groups are part of the choice and have none."""
+        dev = _gpu(logits)
+        if expert.dim() != 2 or logits.dim() != 2:
+            raise _abi.GrimoireError("logits [T][E], expert [T][K]")
+        T, K = shape = expert.shape
+        E = logits.shape[1]
+        lp, b16, stride = _rows(logits, "logits", E, T)
+        dp, d16, dstride = _rows(dlogits, "dlogits", E, T)
+        if d16 != b16 or dlogits.get_device() != dev:
+            raise _abi.GrimoireError("dlogits: of the logits' type, on their device")
+        _launch(dev, stream, lib().grimoire_moe_router_scores_grad, "router_scores_grad", self._ref, lp, b16, stride,
+                _flat(expert, "expert", shape, _I32, dev), _flat(dweight, "dweight", shape, _F32, dev), dp, dstride, T,
+                E, K)
 
 
 class BlockNorm:
@@ -523,6 +546,147 @@ class Lora:
         """h [T][N/2] = silu(gate) * up of the gate|up projection base
         [T][N] plus the adapters' product of x."""
         self._call(self._swiglu, "lora_swiglu", row_slot, x, base, h, self._KN[1] // 2, stream)
+
+
+# ------------------------------------------- tokens to expert order and back
+
+class TokenSort:
+    """Tokens to rows in expert order, with weights applied before the experts
+    (grimoire_moe_sort_rows), and its gradient.  Holds the workspace of up to
+    max_tokens tokens: calls of one object must not overlap, and it stays while
+    a graph or a stream other than the one it was made on has calls of it."""
+
+    def __init__(self, num_experts: int, top_k: int, max_tokens: int, device="cuda"):
+        self.num_experts, self.top_k, self.max_tokens = num_experts, top_k, max_tokens
+        nbytes = route_workspace_bytes(max_tokens, top_k, num_experts)
+        self._workspace = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        _dev(self._workspace)
+        self.dev = self._workspace.get_device()
+        self._ws = (self._workspace.data_ptr(), nbytes)
+        self._sort, self._grad = lib().grimoire_moe_sort_rows, lib().grimoire_moe_sort_rows_grad
+
+    workspace = property(lambda self: self._workspace)
+
+    def __call__(self, ids, x, rows, counts, offsets, inverse, weight=None, perm_token=None, stream=None):
+        """rows[inverse[t, s]] = weight[t, s] * x[t] for ids int32 [T][K]:
+        x [T][H] (rows may lie apart) and rows [T*K][H] fp32 or bf16, weight
+        fp32 [T][K] or None, counts and offsets int32 [E], inverse int32 [T*K]
+        or [T][K]; perm_token int32 [T*K] gets each row's token."""
+        dev, E, K = self.dev, self.num_experts, self.top_k
+        if x.dim() != 2 or x.get_device() != dev:
+            raise _abi.GrimoireError("x: [T][H] on the workspace's device")
+        T, H = x.shape
+        if T > self.max_tokens:
+            raise _abi.GrimoireError("more tokens than the workspace was sized for")
+        xp, x16, xs = _rows(x, "x", H, T)
+        _launch(dev, stream, self._sort, "sort_rows", _flat(ids, "ids", (T, K), _I32, dev), xp, x16, xs,
+                _flat(weight, "weight", (T, K), _F32, dev), _flat(rows, "rows", (T * K, H), _FB16, dev),
+                rows.dtype is not _f32, _flat(counts, "counts", (E,), _I32, dev),
+                _flat(offsets, "offsets", (E,), _I32, dev), _routes(inverse, "inverse", T, K, dev),
+                _flat(perm_token, "perm_token", (T * K,), _I32, dev), T, H, E, K, *self._ws)
+
+    def grad(self, drows, inverse, dx, x=None, weight=None, dweight=None, stream=None):
+        """dx[t] = sum_s weight[t, s] * drows[inverse[t, s]], and with weights
+        dweight[t, s] = <drows[inverse[t, s]], x[t]>: drows [R][H], x and dx
+        [T][H] (rows may lie apart) fp32 or bf16; x, weight and dweight fp32
+        [T][K] together or None."""
+        dev, K = self.dev, self.top_k
+        if dx.dim() != 2 or drows.dim() != 2 or dx.get_device() != dev:
+            raise _abi.GrimoireError("drows [R][H], dx [T][H] on the workspace's device")
+        T, H = dx.shape
+        R = drows.shape[0]
+        dp, d16, ds = _rows(dx, "dx", H, T)
+        xp, x16, xs = (None, 0, 0) if x is None else _rows(x, "x", H, T)
+        if x is not None and x.get_device() != dev:
+            raise _abi.GrimoireError("x: on another device than dx")
+        _launch(dev, stream, self._grad, "sort_rows_grad", _flat(drows, "drows", (R, H), _FB16, dev),
+                drows.dtype is not _f32, R, _routes(inverse, "inverse", T, K, dev),
+                _flat(weight, "weight", (T, K), _F32, dev), xp, x16, xs, dp, d16, ds,
+                _flat(dweight, "dweight", (T, K), _F32, dev), T, K, H)
+
+
+def combine_grad(dy, rows, inverse, route_weight, drows, dweight, shared=None, gate=None, dshared=None, dgate=None,
+                 stream=None):
+    """The gradient of the combine (grimoire_moe_combine_grad): of y[t] =
+    sum_s route_weight[t, s] * rows[inverse[t, s]] + gate[t] * shared[t] to the
+    rows ([R][H], as they lie, those of no route left alone), the weights fp32
+    [T][K], shared [T][H] and gate fp32 [T].  dy [T][H] (rows may lie apart),
+    rows and shared fp32 or bf16; drows and dshared have the types of rows and
+    shared."""
+    dev = _gpu(dy)
+    if dy.dim() != 2 or rows.dim() != 2 or route_weight.dim() != 2:
+        raise _abi.GrimoireError("dy [T][H], rows [R][H], route_weight [T][K]")
+    T, H = dy.shape
+    R, K = rows.shape[0], route_weight.shape[1]
+    yp, y16, ys = _rows(dy, "dy", H, T)
+    sp = _flat(shared, "shared", (T, H), _FB16, dev)
+    s16 = shared is not None and shared.dtype is not _f32
+    _launch(dev, stream, lib().grimoire_moe_combine_grad, "combine_grad", yp, y16, ys,
+            _flat(rows, "rows", (R, H), _FB16, dev), rows.dtype is not _f32, R,
+            _routes(inverse, "inverse", T, K, dev), _flat(route_weight, "route_weight", (T, K), _F32, dev),
+            _flat(drows, "drows", (R, H), _B16 if rows.dtype is not _f32 else _F32, dev),
+            _flat(dweight, "dweight", (T, K), _F32, dev), sp, s16, _flat(gate, "gate", (T,), _F32, dev),
+            _flat(dshared, "dshared", (T, H), _B16 if s16 else _F32, dev), _flat(dgate, "dgate", (T,), _F32, dev), T, K,
+            H)
+
+
+# ------------------------------------------------------- 4-bit projections
+
+class Projection4:
+    """A dense projection with 4-bit weights (grimoire_proj4 /
+    grimoire_proj4_swiglu) for up to max_rows rows: weight is an INT4, INT4_F16
+    or MXFP4 `Weight` [N][K] on the GPU, whose tensors stay as they are.  Calls
+    of one object must not overlap."""
+
+    def __init__(self, weight: Weight, max_rows: int):
+        _dev(weight.payload)
+        self.dev = weight.payload.get_device()
+        N, K, g = weight.N, weight.K, weight.row_scales
+        if weight.fmt not in (_abi.FMT_INT4, _abi.FMT_INT4_F16, _abi.FMT_MXFP4):
+            raise _abi.GrimoireError(f"weight format {weight.fmt}: INT4, INT4_F16 or MXFP4")
+        if weight.payload.dim() != 2 or weight.scales is None:
+            raise _abi.GrimoireError("weight: payload [N][bytes of a row] and scales")
+        bits = (torch.uint8,) if weight.fmt == _abi.FMT_MXFP4 else (_i16, _b16, torch.float16)
+        _flat(weight.payload, "payload", (N, weight.row_bytes), (torch.uint8,), self.dev)
+        _flat(weight.scales, "scales", (N, g), bits, self.dev)
+        _flat(weight.zeros, "zeros", (N, g), (torch.uint8,), self.dev)
+        self._weight, self._KN, self.max_rows = weight, (K, N), max_rows
+        self._keep = (weight.payload, weight.scales, weight.zeros)
+        self.struct = weight.struct()
+        self._ref = C.byref(self.struct)
+        nbytes = int(lib().grimoire_proj4_workspace_bytes(self._ref, max_rows))
+        self._workspace = torch.empty(nbytes, dtype=torch.uint8, device=weight.payload.device) if nbytes else None
+        self._ws = (_p(self._workspace), nbytes)
+        self._plain, self._swiglu = lib().grimoire_proj4, lib().grimoire_proj4_swiglu
+
+    weight = property(lambda self: self._weight)
+    workspace = property(lambda self: self._workspace)
+
+    def _x(self, x, y, width):
+        if x.dim() != 2:
+            raise _abi.GrimoireError("x: [T][K]")
+        T = x.shape[0]
+        if T > self.max_rows:
+            raise _abi.GrimoireError("more rows than the workspace was sized for")
+        if x.get_device() != self.dev or y.get_device() != self.dev:
+            raise _abi.GrimoireError("x, output and weight on different devices")
+        return T, _rows(x, "x", self._KN[0], T), _rows(y, "output", width, T)
+
+    def __call__(self, x, y, base=None, stream=None):
+        """y = x W^T (+ base): x [T][K], y and base [T][N] fp32 or bf16, rows
+        may lie apart; base may be y."""
+        T, xr, yr = self._x(x, y, self._KN[1])
+        br = (None, 0, 0)
+        if base is not None:
+            br = _rows(base, "base", self._KN[1], T)
+            if base.get_device() != self.dev:
+                raise _abi.GrimoireError("base: on another device than the weight")
+        _launch(self.dev, stream, self._plain, "proj4", self._ref, *xr, *br, *yr, T, *self._ws)
+
+    def swiglu(self, x, h, stream=None):
+        """h [T][N/2] = silu(gate) * up of the gate|up projection x W^T."""
+        T, xr, hr = self._x(x, h, self._KN[1] // 2)
+        _launch(self.dev, stream, self._swiglu, "proj4_swiglu", self._ref, *xr, *hr, T, *self._ws)
 
 
 # ------------------------------------------------------------------- layer

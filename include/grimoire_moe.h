@@ -206,6 +206,24 @@ int grimoire_moe_router_scores(void* stream, const grim_score_params* p, const v
                                int logits_bf16, int64_t row_stride, int tokens, int n_experts,
                                int top_k, int32_t* out_expert, float* out_weight);
 
+/* The gradient of those weights to the logits.  With s the scores, u_k = s of
+ * pick k = expert[t][k], g_k = scaling * dweight[t][k]:
+ *   normalize: du_k = (g_k - sum_j p_j g_j) / Z, p = u / Z, Z = sum u;
+ *   else du_k = g_k.
+ *   softmax: dlogits_e = s_e ([e picked] du_e - sum_k u_k du_k) (with
+ *   normalize the sum is 0: exact zeros where nothing was picked);
+ *   sigmoid: s_e (1 - s_e) [e picked] du_e.
+ * The choice has no gradient: bias and groups in p are not read.  Picks
+ * outside [0, n_experts) (slots no expert was left for) are left out, an
+ * expert picked twice gets the sum.  An expert whose logit is NaN or -inf has
+ * score and gradient 0; +inf counts as the largest finite logit.  dlogits:
+ * rows of the logits' type, d_stride elements apart, every element written;
+ * it may be the logits themselves (same stride).  Sums are fp32. */
+int grimoire_moe_router_scores_grad(void* stream, const grim_score_params* p, const void* logits,
+                                    int logits_bf16, int64_t row_stride, const int32_t* expert,
+                                    const float* dweight, void* dlogits, int64_t d_stride, int tokens,
+                                    int n_experts, int top_k);
+
 /* ------------------------------------------------------------------------
  * Decode / batched-decode expert products (slot form).  h holds
  * [M][KS][I] fp32, KS = top_k (+1 with the shared expert, whose
@@ -331,6 +349,48 @@ int grimoire_moe_combine(void* stream, const uint16_t* src, const int32_t* inver
                          const float* route_weight, const uint16_t* shared_src,
                          const float* gate, float* dst, int tokens, int top_k, int hidden);
 
+/* Tokens to rows in expert order, with weights applied before the experts,
+ * and its gradient; the gradient of the combine.  No counterpart in the
+ * reference, whose dispatch copies rows as bf16 and trains nothing.
+ *   sort_rows:       rows[inverse[t][s]] = weight[t][s] * x[t]  (weight NULL:
+ *                    x[t]), inverse, counts, offsets and perm_token as
+ *                    grimoire_moe_route_grouped; rows [tokens * top_k][hidden];
+ *                    rows behind the last route's keep what they hold.
+ *                    tokens == 0 writes counts and offsets (zeros).
+ *   sort_rows_grad:  dx[t] = sum_s weight[t][s] * drows[inverse[t][s]];
+ *                    dweight[t][s] = <drows[inverse[t][s]], x[t]>.  weight, x
+ *                    and dweight come together, or are NULL (weights of 1).
+ *   combine_grad:    of y[t] = sum_s weight[t][s] * rows[inverse[t][s]] +
+ *                    gate[t] * shared[t]:  drows[inverse[t][s]] = weight[t][s]
+ *                    * dy[t], dweight[t][s] = <dy[t], rows[inverse[t][s]]>,
+ *                    dshared[t] = gate[t] * dy[t] (gate NULL: dy[t]),
+ *                    dgate[t] = <dy[t], shared[t]>.  dshared comes with
+ *                    shared, dgate with gate; gate needs shared.
+ * A route whose expert is outside [0, num_experts), or whose inverse is outside
+ * [0, n_rows), has no row: it adds nothing, its dweight is 0.  Rows that no
+ * route names keep what drows holds; the routes of one call name different
+ * rows (of several routes to one row, one writes it).  x, dx and dy: fp32 or
+ * bf16, rows an own distance of elements apart (a multiple of 4, <= 2^28); the other
+ * rows lie one behind the other.  drows has the rows' type, dshared shared's.
+ * Sums are fp32, rounded once.  hidden % 4 == 0, top_k <= 16; fp32 rows
+ * 16-byte, bf16 rows 8-byte aligned (with 16 bytes and hidden and distances a
+ * multiple of 8, bf16 is accessed 16 bytes at a time).  No output overlaps
+ * another argument.  The workspace is grimoire_moe_route_workspace_bytes. */
+int grimoire_moe_sort_rows(void* stream, const int32_t* ids, const void* x, int x_bf16, int64_t x_stride,
+                           const float* weight, void* rows, int rows_bf16, int32_t* counts,
+                           int32_t* offsets, int32_t* inverse, int32_t* perm_token, int tokens,
+                           int hidden, int num_experts, int top_k, void* workspace,
+                           size_t workspace_bytes);
+int grimoire_moe_sort_rows_grad(void* stream, const void* drows, int rows_bf16, int64_t n_rows,
+                                const int32_t* inverse, const float* weight, const void* x, int x_bf16,
+                                int64_t x_stride, void* dx, int dx_bf16, int64_t dx_stride,
+                                float* dweight, int tokens, int top_k, int hidden);
+int grimoire_moe_combine_grad(void* stream, const void* dy, int dy_bf16, int64_t dy_stride,
+                              const void* rows, int rows_bf16, int64_t n_rows, const int32_t* inverse,
+                              const float* weight, void* drows, float* dweight, const void* shared,
+                              int shared_bf16, const float* gate, void* dshared, float* dgate,
+                              int tokens, int top_k, int hidden);
+
 /* Combine fused with the residual add and the next RMSNorm.  Per token t:
  * v = h[t] + shared[t] (shared NULL = 0), then v = fma(route_weight[t,s],
  * routed[inverse[t,s]], v) in slot order (inverse -1 skips the slot);
@@ -453,6 +513,35 @@ int grimoire_lora_swiglu(void* stream, const grim_lora* L, const int32_t* row_sl
                          int x_bf16, int64_t x_stride, const void* base, int base_bf16,
                          int64_t base_stride, void* h, int h_bf16, int64_t h_stride, int rows,
                          void* workspace, size_t workspace_bytes);
+
+/* ------------------------------------------------------------------------
+ * A dense projection [N][K] with 4-bit weights for a few rows (one token, a
+ * batch of decoding sequences, a draft): the shared expert's or another
+ * projection of a layer that is built from single operators.  The reference
+ * runs these through gemv_any (src/grimoire.cpp:15364).  w: GRIM_FMT_INT4 or
+ * GRIM_FMT_INT4_F16 in groups of 32, 64, 128 or 256, or GRIM_FMT_MXFP4, as
+ * described at enum grim_fmt.
+ *   proj4:         y[t] = base[t] + W x[t] (base NULL: W x[t])
+ *   proj4_swiglu:  N = 2I, gate rows first: h[t][i] = silu(v[i]) * v[I + i],
+ *                  v = W x[t]
+ * x [rows][K], base and y [rows][N], h [rows][I]: fp32 or bf16 rows, *_stride
+ * elements apart (x a multiple of 8, 16-byte aligned; at most 2^28).  y may be
+ * base (same type and stride) and overlaps nothing else; rows at one distance
+ * may lie beside each other in one buffer.  Codes and fp32 or bf16 activations
+ * are multiplied exactly, sums are fp32.  A row of x with an infinity or a NaN
+ * gives NaN or infinities in its own row alone; finite x should stay below
+ * 1e36 (codes are multiplied as 16 + q).  Any number of rows; the weights are
+ * read again for every 32 (bf16) or 10 (fp32) of them.
+ * The workspace (16-byte aligned, no initial contents, apart from every other
+ * argument) may be NULL where grimoire_proj4_workspace_bytes is 0; calls that
+ * share one must not overlap. */
+size_t grimoire_proj4_workspace_bytes(const grim_quant_weight* w, int rows);
+int grimoire_proj4(void* stream, const grim_quant_weight* w, const void* x, int x_bf16, int64_t x_stride,
+                   const void* base, int base_bf16, int64_t base_stride, void* y, int y_bf16,
+                   int64_t y_stride, int rows, void* workspace, size_t workspace_bytes);
+int grimoire_proj4_swiglu(void* stream, const grim_quant_weight* w, const void* x, int x_bf16,
+                          int64_t x_stride, void* h, int h_bf16, int64_t h_stride, int rows,
+                          void* workspace, size_t workspace_bytes);
 
 /* ------------------------------------------------------------------------
  * Expert-weight ingestion: one checkpoint projection [out][in] of one expert
