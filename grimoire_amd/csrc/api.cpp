@@ -736,19 +736,18 @@ int grimoire_moe_combine_grad(void* stream, const void* dy, int dy_bf16, int64_t
 }
 
 size_t grimoire_proj4_workspace_bytes(const grim_quant_weight* w, int rows) {
-    (void)w;
-    (void)rows;
-    return 0;
+    return w && rows > 0 ? proj4_workspace_bytes(rows) : 0;
 }
 
 static int proj4_common(void* stream, const grim_quant_weight* w, const void* x, int x_bf16, int64_t x_stride,
                         const void* base, int base_bf16, int64_t base_stride, void* y, int y_bf16,
-                        int64_t y_stride, int rows, int glu) {
+                        int64_t y_stride, int rows, void* ws, size_t ws_bytes, int glu) {
     if (rows <= 0) return GRIM_OK;
     if (!w || !x || !y) return fail(GRIM_ERR_ARG, "null pointer");
     if (w->fmt != GRIM_FMT_INT4 && w->fmt != GRIM_FMT_INT4_F16 && w->fmt != GRIM_FMT_MXFP4)
         return fail(GRIM_ERR_FORMAT, "projection: format %d (INT4, INT4_F16 or MXFP4)", w->fmt);
     if (w->K <= 0 || w->N <= 0 || (glu && w->N % 2)) return fail(GRIM_ERR_SHAPE, "N=%d K=%d", w->N, w->K);
+    if (rows > kProj4MaxRows) return fail(GRIM_ERR_SHAPE, "rows=%d (<= %d)", rows, kProj4MaxRows);
     if (int r = check_weight(w, "projection", w->N, w->K)) return r;
     if (w->fmt != GRIM_FMT_MXFP4 && !aligned(w->scales, 2)) return fail(GRIM_ERR_ARG, "scales alignment");
     const int width = glu ? w->N / 2 : w->N;
@@ -760,30 +759,32 @@ static int proj4_common(void* stream, const grim_quant_weight* w, const void* x,
         return fail(GRIM_ERR_ARG, "x 16-byte, y and base an element's alignment");
     const RowSpan out = row_span(y, y_bf16, y_stride, width, rows);
     const RowSpan add = row_span(base, base_bf16, base_stride, width, rows);
+    const size_t need = proj4_workspace_bytes(rows);
+    if (!ws || ws_bytes < need) return fail(GRIM_ERR_WORKSPACE, "projection workspace too small (need %zu)", need);
+    if (!aligned(ws, 16)) return fail(GRIM_ERR_ARG, "workspace not 16-byte aligned");
+    const RowSpan work = whole(ws, int64_t(need));
     const int64_t sb = int64_t(w->N) * w->row_scales;
-    if (any_shared({out}, {row_span(x, x_bf16, x_stride, w->K, rows), whole(w->payload, w->N * w->row_bytes),
+    if (any_shared({out, work}, {row_span(x, x_bf16, x_stride, w->K, rows), whole(w->payload, w->N * w->row_bytes),
                            whole(w->scales, w->fmt == GRIM_FMT_MXFP4 ? sb : 2 * sb), whole(w->zeros, sb)}) ||
-        (share_memory(out, add) && (!same_rows(out, add) || !base_bf16 != !y_bf16)))
+        share_memory(work, add) || (share_memory(out, add) && (!same_rows(out, add) || !base_bf16 != !y_bf16)))
         return fail(GRIM_ERR_ARG, "the output overlaps another argument");
     Proj4Args a{view(*w), w->fmt, w->N, w->K, x, base, y, x_stride, base_stride, y_stride, x_bf16 ? 1 : 0,
-                base_bf16 ? 1 : 0, y_bf16 ? 1 : 0, rows, glu};
+                base_bf16 ? 1 : 0, y_bf16 ? 1 : 0, rows, glu, ws};
     return status(proj4_launch(S(stream), a));
 }
 
 int grimoire_proj4(void* stream, const grim_quant_weight* w, const void* x, int x_bf16, int64_t x_stride,
                    const void* base, int base_bf16, int64_t base_stride, void* y, int y_bf16,
                    int64_t y_stride, int rows, void* workspace, size_t workspace_bytes) {
-    (void)workspace;
-    (void)workspace_bytes;
-    return proj4_common(stream, w, x, x_bf16, x_stride, base, base_bf16, base_stride, y, y_bf16, y_stride, rows, 0);
+    return proj4_common(stream, w, x, x_bf16, x_stride, base, base_bf16, base_stride, y, y_bf16, y_stride, rows,
+                        workspace, workspace_bytes, 0);
 }
 
 int grimoire_proj4_swiglu(void* stream, const grim_quant_weight* w, const void* x, int x_bf16,
                           int64_t x_stride, void* h, int h_bf16, int64_t h_stride, int rows,
                           void* workspace, size_t workspace_bytes) {
-    (void)workspace;
-    (void)workspace_bytes;
-    return proj4_common(stream, w, x, x_bf16, x_stride, nullptr, 0, 0, h, h_bf16, h_stride, rows, 1);
+    return proj4_common(stream, w, x, x_bf16, x_stride, nullptr, 0, 0, h, h_bf16, h_stride, rows, workspace,
+                        workspace_bytes, 1);
 }
 
 size_t grimoire_lora_workspace_bytes(const grim_lora* L, int rows) {

@@ -530,11 +530,12 @@ int grimoire_lora_swiglu(void* stream, const grim_lora* L, const int32_t* row_sl
  * may lie beside each other in one buffer.  Codes and fp32 or bf16 activations
  * are multiplied exactly, sums are fp32.  A row of x with an infinity or a NaN
  * gives NaN or infinities in its own row alone; finite x should stay below
- * 1e36 (codes are multiplied as 16 + q).  Any number of rows; the weights are
- * read again for every 32 (bf16) or 10 (fp32) of them.
- * The workspace (16-byte aligned, no initial contents, apart from every other
- * argument) may be NULL where grimoire_proj4_workspace_bytes is 0; calls that
- * share one must not overlap. */
+ * 1e36 (codes are multiplied as 16 + q).  Up to 2^19 rows; the weights are
+ * read again for every 64 (bf16) or 16 (fp32) of them.
+ * The workspace holds grimoire_proj4_workspace_bytes for up to `rows` rows
+ * (16-byte aligned, no initial contents, apart from every other argument);
+ * calls that share one must not overlap: two graphs that hold it run one after
+ * the other. */
 size_t grimoire_proj4_workspace_bytes(const grim_quant_weight* w, int rows);
 int grimoire_proj4(void* stream, const grim_quant_weight* w, const void* x, int x_bf16, int64_t x_stride,
                    const void* base, int base_bf16, int64_t base_stride, void* y, int y_bf16,

@@ -319,4 +319,6 @@ def test_host_refusals_on_the_gpu_objects(gpu):
         proj(shared[:4], shared[:4, :16])                                             # output inside x
     lib = _abi.lib()
     assert lib.grimoire_proj4(None, C.byref(proj.struct), x.data_ptr(), 0, 64, None, 0, 0, w.payload.data_ptr(), 0, 16, 4,
-                              None, 0) == _abi.ERR_ARG
+                              *proj._ws) == _abi.ERR_ARG
+    assert lib.grimoire_proj4(None, C.byref(proj.struct), x.data_ptr(), 0, 64, None, 0, 0, y.data_ptr(), 0, 16, 4, None,
+                              0) == _abi.ERR_WORKSPACE

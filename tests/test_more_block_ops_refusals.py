@@ -19,18 +19,19 @@ def weight(**kw):
 
 
 def proj(w=None, **kw):
-    d = dict(x=P[3], x16=0, xs=256, base=None, b16=0, bs=0, y=P[4], y16=0, ys=64, rows=4)
+    d = dict(x=P[3], x16=0, xs=256, base=None, b16=0, bs=0, y=P[4], y16=0, ys=64, rows=4, ws=P[6], n=1 << 24)
     d.update(kw)
     w = weight() if w is None else w
     return _abi.lib().grimoire_proj4(None, C.byref(w), d["x"], d["x16"], d["xs"], d["base"], d["b16"], d["bs"], d["y"],
-                                     d["y16"], d["ys"], d["rows"], None, 0)
+                                     d["y16"], d["ys"], d["rows"], d["ws"], d["n"])
 
 
 def glu(w=None, **kw):
-    d = dict(x=P[3], xs=256, h=P[4], hs=32, rows=4)
+    d = dict(x=P[3], xs=256, h=P[4], hs=32, rows=4, ws=P[6], n=1 << 24)
     d.update(kw)
     w = weight() if w is None else w
-    return _abi.lib().grimoire_proj4_swiglu(None, C.byref(w), d["x"], 0, d["xs"], d["h"], 0, d["hs"], d["rows"], None, 0)
+    return _abi.lib().grimoire_proj4_swiglu(None, C.byref(w), d["x"], 0, d["xs"], d["h"], 0, d["hs"], d["rows"], d["ws"],
+                                            d["n"])
 
 
 @pytest.mark.parametrize("w,status", [
@@ -50,7 +51,8 @@ def test_weights(w, status):
     (dict(x=P[3] + 8), ARG), (dict(y=P[4] + 2), ARG), (dict(base=P[5] + 1, bs=64), ARG),
     (dict(y=P[3]), ARG), (dict(y=P[0]), ARG), (dict(y=P[1]), ARG), (dict(y=P[2]), ARG),
     (dict(base=P[4], bs=128), ARG), (dict(base=P[4], bs=64, b16=1), ARG), (dict(base=P[4] + 4, bs=64), ARG),
-    (dict(x=P[4] + 512, y=P[4]), ARG)])
+    (dict(x=P[4] + 512, y=P[4]), ARG), (dict(ws=None), WS), (dict(n=1024), WS), (dict(ws=P[6] + 8), ARG),
+    (dict(ws=P[3]), ARG), (dict(ws=P[4]), ARG), (dict(ws=P[0]), ARG), (dict(ws=P[2]), ARG), (dict(base=P[6], bs=64), ARG)])
 def test_projection_arguments(kw, status):
     assert proj(**kw) == status
 
@@ -60,7 +62,12 @@ def test_projection_no_rows_and_odd_glu():
     assert glu(weight(N=63)) == SHAPE
     assert glu(hs=31) == SHAPE
     assert glu(h=P[3]) == ARG
-    assert _abi.lib().grimoire_proj4(None, None, P[3], 0, 256, None, 0, 0, P[4], 0, 64, 4, None, 0) == ARG
+    assert _abi.lib().grimoire_proj4(None, None, P[3], 0, 256, None, 0, 0, P[4], 0, 64, 4, P[6], 1 << 24) == ARG
+    assert _abi.lib().grimoire_proj4_workspace_bytes(None, 4) == 0
+    w = weight()
+    n = [_abi.lib().grimoire_proj4_workspace_bytes(C.byref(w), r) for r in (-1, 0, 1, 4, 64, 65, 1 << 20)]
+    assert n[0] == n[1] == 0 and 0 < n[2] < n[3] < n[4] == n[5] == n[6]
+    assert proj(n=n[3], y=None) == ARG and proj(n=n[3] - 1) == WS
 
 
 def sort(**kw):
