@@ -190,6 +190,7 @@ SIGNATURES = {
     "grimoire_block_norm": (I32, [P, C.POINTER(BlockNormParams), P, I32, P, P, I32, I64, P, P, P, I32, I32]),
     "grimoire_moe_block_norm": (I32, [P, C.POINTER(BlockNormParams), P, I32, P, P, I32, P, P, P, P, P, P, I32,
                                       I32, I32]),
+    "grimoire_moe_sort_workspace_bytes": (SZ, [I32, I32, I32]),
     "grimoire_moe_sort_rows": (I32, [P, P, P, I32, I64, P, P, I32, P, P, P, P, I32, I32, I32, I32, P, SZ]),
     "grimoire_moe_sort_rows_grad": (I32, [P, P, I32, I64, P, P, P, I32, I64, P, I32, I64, P, I32, I32, I32]),
     "grimoire_moe_combine_grad": (I32, [P, P, I32, I64, P, I32, I64, P, P, P, P, P, I32, P, P, P, I32, I32, I32]),

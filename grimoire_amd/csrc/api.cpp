@@ -652,6 +652,10 @@ static int route_shape(int tokens, int top_k, int hidden) {
     return GRIM_OK;
 }
 
+size_t grimoire_moe_sort_workspace_bytes(int tokens, int top_k, int num_experts) {
+    return sort_rows_workspace_bytes(tokens, top_k, num_experts);
+}
+
 int grimoire_moe_sort_rows(void* stream, const int32_t* ids, const void* x, int x_bf16, int64_t x_stride,
                            const float* weight, void* rows, int rows_bf16, int32_t* counts,
                            int32_t* offsets, int32_t* inverse, int32_t* perm_token, int tokens,
@@ -673,9 +677,9 @@ int grimoire_moe_sort_rows(void* stream, const int32_t* ids, const void* x, int 
     if (!stride_ok(x_stride, hidden, 4)) return fail(GRIM_ERR_SHAPE, "x_stride=%lld", (long long)x_stride);
     if (!rows_aligned(x, x_bf16) || !rows_aligned(rows, rows_bf16))
         return fail(GRIM_ERR_ARG, "fp32 rows 16-byte, bf16 rows 8-byte alignment");
-    const size_t need = dispatch_workspace_bytes(tokens, top_k, num_experts);
+    const size_t need = sort_rows_workspace_bytes(tokens, top_k, num_experts);
     if (!workspace || workspace_bytes < need)
-        return fail(GRIM_ERR_WORKSPACE, "dispatch workspace too small (need %zu)", need);
+        return fail(GRIM_ERR_WORKSPACE, "sort workspace too small (need %zu)", need);
     if (!aligned(workspace, 4)) return fail(GRIM_ERR_ARG, "workspace alignment");
     if (any_shared({row_span(rows, rows_bf16, hidden, hidden, n), whole(counts, eb), whole(offsets, eb),
                     whole(inverse, n * 4), whole(perm_token, n * 4), whole(workspace, int64_t(need))},

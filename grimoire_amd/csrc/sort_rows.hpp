@@ -16,7 +16,7 @@ struct SortRowsArgs {
     int32_t *counts, *offsets, *inverse, *perm_token;   // perm_token may be null
     int x_bf16, rows_bf16;
     int T, K, E, H;
-    void* workspace;         // dispatch_workspace_bytes
+    void* workspace;         // sort_rows_workspace_bytes
 };
 
 // dx[t] = sum_s w[t][s] * drows[inverse[t][s]],  dw[t][s] = <drows[inverse[t][s]], x[t]>
@@ -54,6 +54,7 @@ struct CombineGradArgs {
 
 constexpr int kSortMaxE = 16384;     // a count a byte quad in 64 KiB of LDS
 
+size_t sort_rows_workspace_bytes(int T, int K, int E);
 hipError_t sort_rows_launch(hipStream_t st, const SortRowsArgs& a);
 hipError_t sort_grad_launch(hipStream_t st, const SortGradArgs& a);
 hipError_t combine_grad_launch(hipStream_t st, const CombineGradArgs& a);

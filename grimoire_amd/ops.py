@@ -558,7 +558,7 @@ class TokenSort:
 
     def __init__(self, num_experts: int, top_k: int, max_tokens: int, device="cuda"):
         self.num_experts, self.top_k, self.max_tokens = num_experts, top_k, max_tokens
-        nbytes = route_workspace_bytes(max_tokens, top_k, num_experts)
+        nbytes = int(lib().grimoire_moe_sort_workspace_bytes(max_tokens, top_k, num_experts))
         self._workspace = torch.empty(nbytes, dtype=torch.uint8, device=device)
         _dev(self._workspace)
         self.dev = self._workspace.get_device()

@@ -375,7 +375,10 @@ int grimoire_moe_combine(void* stream, const uint16_t* src, const int32_t* inver
  * Sums are fp32, rounded once.  hidden % 4 == 0, top_k <= 16; fp32 rows
  * 16-byte, bf16 rows 8-byte aligned (with 16 bytes and hidden and distances a
  * multiple of 8, bf16 is accessed 16 bytes at a time).  No output overlaps
- * another argument.  The workspace is grimoire_moe_route_workspace_bytes. */
+ * another argument.  sort_rows takes a workspace (4-byte aligned, no initial
+ * contents; calls that share one must not overlap) of
+ * grimoire_moe_sort_workspace_bytes for up to `tokens` tokens. */
+size_t grimoire_moe_sort_workspace_bytes(int tokens, int top_k, int num_experts);
 int grimoire_moe_sort_rows(void* stream, const int32_t* ids, const void* x, int x_bf16, int64_t x_stride,
                            const float* weight, void* rows, int rows_bf16, int32_t* counts,
                            int32_t* offsets, int32_t* inverse, int32_t* perm_token, int tokens,
