@@ -95,14 +95,9 @@ __device__ __forceinline__ void put_chunk(uint8_t* to, u32x4 lo, u32x4 hi, bool 
 }
 
 template <bool XB>
-__device__ __forceinline__ void get_chunk(const void* x, int64_t at, u32x4& lo, u32x4& hi) {
-    if constexpr (XB) {
-        lo = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(x) + at);
-    } else {
-        const u32x4* f = reinterpret_cast<const u32x4*>(static_cast<const float*>(x) + at);
-        lo = f[0];
-        hi = f[1];
-    }
+__device__ __forceinline__ void get_chunk(const uint8_t* at, u32x4& lo, u32x4& hi) {
+    lo = reinterpret_cast<const u32x4*>(at)[0];
+    if constexpr (!XB) hi = reinterpret_cast<const u32x4*>(at)[1];
 }
 
 // GS: group size of INT4 (32, 64, 128; 256 reads each scale twice), 0: MXFP4.
@@ -115,9 +110,9 @@ __global__ __launch_bounds__(kWaves * 64, CT == 4 ? 2 : 4) void proj4_kernel(Pro
     constexpr int L = XB ? 1 : 3;                      // pieces of a row of x
     constexpr int TR = XB ? 16 : 4;                    // its rows in a tile; column 4 t + l is piece l
     constexpr int kFetch = XB ? 8 : 4;                 // a lane's chunks of x in flight
-    // sums of x over a group: of one tile one more product a step, of several
-    // formed once and kept in the LDS
-    constexpr bool kSums = GS != 0 && CT > 1;
+    // sums of x over a group: of one or two tiles one more product a step (the
+    // matrix cores wait for the decoding), of four formed once and kept in the LDS
+    constexpr bool kSums = GS != 0 && CT > 2;
     const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, q = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int KS = 1 << p.ks, kg = wave & (KS - 1), rg = wave >> p.ks, RG = kWaves >> p.ks;
@@ -137,7 +132,11 @@ __global__ __launch_bounds__(kWaves * 64, CT == 4 ? 2 : 4) void proj4_kernel(Pro
     // An item: kSeg blocks of a tile's 16 rows; a lane's word of block u.
     u32x4 ring[kSeg];
     const uint8_t* row_at;
-    auto tile_rows = [&](int set) { row_at = a.w.payload + weight_row(set * RG + rg, here(r)) * a.w.row_bytes; };
+    int64_t s_row;                                     // of the scales this lane loads
+    auto tile_rows = [&](int set) {
+        row_at = a.w.payload + weight_row(set * RG + rg, here(r)) * a.w.row_bytes;
+        s_row = weight_row(set * RG + rg, here(lane) >> 2) * a.w.row_scales;
+    };
     auto load_w = [&](int u, int first) {
         // a lane past the row's end (x is 0 there) reads its start
         const int b = min(first + u, p.nb - 1), k = b * kBlk + q * 32;
@@ -145,10 +144,9 @@ __global__ __launch_bounds__(kWaves * 64, CT == 4 ? 2 : 4) void proj4_kernel(Pro
     };
     // scales of an item: lane (row lane / 4, block lane % 4), PG of them
     uint32_t sr[PG], zr[PG];
-    auto load_s = [&](int set, int first) {
-        const int srow = here(lane) >> 2, sblk = here(lane) & 3;
-        const int64_t base = weight_row(set * RG + rg, srow) * a.w.row_scales;
-        const int k0 = min(first + sblk, p.nb - 1) * kBlk;
+    auto load_s = [&](int first) {
+        const int64_t base = s_row;
+        const int k0 = min(first + (here(lane) & 3), p.nb - 1) * kBlk;
 #pragma unroll
         for (int e = 0; e < PG; ++e) {
             if constexpr (GS == 0) {
@@ -203,13 +201,17 @@ __global__ __launch_bounds__(kWaves * 64, CT == 4 ? 2 : 4) void proj4_kernel(Pro
     // zeros
     const int rb = nt >= 3 ? 2 : nt - 1, cb = 6 - rb;
     const int tqb = nt <= 4 ? 0 : 32 - __builtin_clz((nt - 1) >> 2);       // log2 of the units along the rows
+    const int size = XB ? 2 : 4;
+    const uint8_t* x_at = static_cast<const uint8_t*>(a.x) + int64_t(t0) * a.x_stride * size;
     auto fetch = [&](u32x4 (&xv)[kFetch][2], int s0, int n, int i) {
         const int cl = here(lane) & ((1 << cb) - 1), tl = here(lane) >> cb;
+        const uint8_t* lane_at = x_at + (int64_t(tl) * a.x_stride + cl * 8) * size;
 #pragma unroll
         for (int j = 0; j < kFetch; ++j) {
-            const int u = i + j * kWaves, c = ((u >> tqb) << cb) + cl, t = ((u & ((1 << tqb) - 1)) << rb) + tl;
-            const int64_t at = int64_t(t0 + min(t, nt - 1)) * a.x_stride + int64_t(min(s0 * kChunks + min(c, n * kChunks - 1), cK - 1)) * 8;
-            get_chunk<XB>(a.x, at, xv[j][0], xv[j][1]);
+            const int u = i + j * kWaves, cu = (u >> tqb) << cb, tu = (u & ((1 << tqb) - 1)) << rb;
+            const bool in = cu + cl < n * kChunks && s0 * kChunks + cu + cl < cK && tu + tl < nt;
+            const int64_t at = (int64_t(tu) * a.x_stride + (s0 * kChunks + cu) * int64_t(8)) * size;   // of every lane
+            get_chunk<XB>(in ? lane_at + at : x_at, xv[j][0], xv[j][1]);       // a lane with none: the first
         }
     };
     auto put = [&](const u32x4 (&xv)[kFetch][2], int s0, int n, int i) {
@@ -267,7 +269,7 @@ __global__ __launch_bounds__(kWaves * 64, CT == 4 ? 2 : 4) void proj4_kernel(Pro
         u32x4 xv[kFetch][2];
         fetch(xv, kb0, n, wave);                       // x first: it is waited for first
         tile_rows(set0);
-        load_s(set0, kb0 + kg * WB);
+        load_s(kb0 + kg * WB);
 #pragma unroll
         for (int u = 0; u < kSeg; ++u) load_w(u, kb0 + kg * WB);
         put(xv, kb0, n, wave);
@@ -313,21 +315,23 @@ __global__ __launch_bounds__(kWaves * 64, CT == 4 ? 2 : 4) void proj4_kernel(Pro
             for (int g = 0; g < PG; ++g) {
                 const float s = ls[(u * PG + g) * 16 + r], z = lz[(u * PG + g) * 16 + r];
                 const uint32_t flip = z < 0.0f ? kSigned : kCodes;
-                f32x4 D[CT], X1 = {0.f, 0.f, 0.f, 0.f};
+                f32x4 D[CT], X1[CT];
 #pragma unroll
-                for (int c = 0; c < CT; ++c) D[c] = f32x4{0.f, 0.f, 0.f, 0.f};
+                for (int c = 0; c < CT; ++c) D[c] = X1[c] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int k = g * KG; k < (g + 1) * KG; ++k) {
                     operands(k);
                     const u32x4 wf = codes16(raw[k], flip);
                     const uint32_t one = 0x3F803F80u;
-                    if constexpr (!kSums) X1 = mfma(xf[k % PRE][0], u32x4{one, one, one, one}, X1);
 #pragma unroll
-                    for (int c = 0; c < CT; ++c) D[c] = mfma(xf[k % PRE][c], wf, D[c]);
+                    for (int c = 0; c < CT; ++c) {
+                        if constexpr (!kSums) X1[c] = mfma(xf[k % PRE][c], u32x4{one, one, one, one}, X1[c]);
+                        D[c] = mfma(xf[k % PRE][c], wf, D[c]);
+                    }
                 }
 #pragma unroll
                 for (int c = 0; c < CT; ++c) {
-                    f32x4 X = X1;
+                    f32x4 X = X1[c];
                     if constexpr (kSums) X = *reinterpret_cast<const f32x4*>(lX + ((b * PG + g) * CT + c) * 16 + q * 4);
 #pragma unroll
                     for (int m = 0; m < 4; ++m)
@@ -362,7 +366,7 @@ __global__ __launch_bounds__(kWaves * 64, CT == 4 ? 2 : 4) void proj4_kernel(Pro
                         if (nset != set) tile_rows(nset);
                     }
                 }
-                load_s(nset, next);
+                load_s(next);
                 // whole items without a branch between their blocks, so that one
                 // block's operands are on their way while another's are used
                 const int valid = min(min(kSeg, WB - item * kSeg), end - in);
@@ -462,7 +466,7 @@ hipError_t proj4_go(hipStream_t st, Proj4Dev& p) {
     p.nb = (a.K + kBlk - 1) / kBlk;
     p.tiles = (p.half + (a.glu ? 7 : 15)) / (a.glu ? 8 : 16);
     const auto up = [](int n, int d) { return (n + d - 1) / d; };
-    const int x_blk = kChunks * (p.tile_rows * L + 1) * 16, X_blk = GS == 0 || CT == 1 ? 0 : PG * CT * 64;
+    const int x_blk = kChunks * (p.tile_rows * L + 1) * 16, X_blk = GS == 0 || CT <= 2 ? 0 : PG * CT * 64;
     const int s_all = kWaves * kSeg * PG * 16 * (GS == 0 ? 4 : 8), red_most = kWaves * CT * TR * 64;
     // blocks whose x fits beside a second work-group
     const int fit = std::max(1, int(kLdsHalf - s_all - red_most) / (x_blk + X_blk));
