@@ -29,14 +29,14 @@ struct Proj4Dev {
     int kw, kw_blocks;        // parts of K by work-groups, and blocks of 128 of one
     int ks, wave_blocks;      // log2 of the waves that share a tile, and blocks of one in a slab
     int nb, slab;             // blocks along K, and of those whose x is in the LDS together
-    int X_at, w_at, s_at, red_at;   // LDS offsets: sums of x, weights, scales, partial sums
+    int s_at, red_at;         // LDS offsets: scales, partial sums
     int half;                 // outputs: N, or N / 2 with glu
 };
 
 // Sums over parts of K are of at most this many (tile of 16 outputs, part of K,
 // work-group's rows of x), whose rows are at most kProj4TileRows.
 constexpr int kProj4MaxRows = 1 << 19;
-constexpr int kProj4Tiles = 4096, kProj4TileRows = 64;
+constexpr int kProj4Tiles = 4096, kProj4TileRows = 32;
 inline size_t proj4_workspace_bytes(int rows) {
     return size_t(kProj4Tiles) * 64 * (rows < kProj4TileRows ? rows : kProj4TileRows);
 }

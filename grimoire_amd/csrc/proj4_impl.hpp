@@ -103,16 +103,13 @@ __device__ __forceinline__ void get_chunk(const uint8_t* at, u32x4& lo, u32x4& h
 // GS: group size of INT4 (32, 64, 128; 256 reads each scale twice), 0: MXFP4.
 // XB: x is bf16.  CT: 16-column tiles of x.
 template <int GS, bool XB, int CT>
-__global__ __launch_bounds__(kWaves * 64, CT == 4 ? 2 : 4) void proj4_kernel(Proj4Dev p) {
+__global__ __launch_bounds__(kWaves * 64, 4) void proj4_kernel(Proj4Dev p) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     const Proj4Args& a = p.a;
     constexpr int PG = GS == 0 ? 4 : kBlk / GS;        // scales of a row and block
     constexpr int L = XB ? 1 : 3;                      // pieces of a row of x
     constexpr int TR = XB ? 16 : 4;                    // its rows in a tile; column 4 t + l is piece l
     constexpr int kFetch = XB ? 8 : 4;                 // a lane's chunks of x in flight
-    // sums of x over a group: of one or two tiles one more product a step (the
-    // matrix cores wait for the decoding), of four formed once and kept in the LDS
-    constexpr bool kSums = GS != 0 && CT > 2;
     const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, q = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int KS = 1 << p.ks, kg = wave & (KS - 1), rg = wave >> p.ks, RG = kWaves >> p.ks;
@@ -179,7 +176,6 @@ __global__ __launch_bounds__(kWaves * 64, CT == 4 ? 2 : 4) void proj4_kernel(Pro
     };
 
     const int xs = (NC + 1) * 16;                      // bytes of a chunk's columns, padded against bank conflicts
-    float* lX = reinterpret_cast<float*>(lds + p.X_at);                     // [block][group][CT][16] sums of x
     // LDS column of this lane in each tile (past the last: the first, not used)
     int col[CT];
 #pragma unroll
@@ -223,7 +219,7 @@ __global__ __launch_bounds__(kWaves * 64, CT == 4 ? 2 : 4) void proj4_kernel(Pro
                 put_chunk<GS, XB>(lds + c * xs + t * L * 16, xv[j][0], xv[j][1], s0 * kChunks + c < cK);
         }
     };
-    // ... the units from i on, and the sums
+    // ... the units from i on
     auto stage = [&](int s0, int n, int i) {
         const int total = ((n * kChunks + (1 << cb) - 1) >> cb) << tqb;
         for (; i < total; i += kFetch * kWaves) {
@@ -232,36 +228,6 @@ __global__ __launch_bounds__(kWaves * 64, CT == 4 ? 2 : 4) void proj4_kernel(Pro
             put(xv, s0, n, i);
         }
         __syncthreads();
-        if constexpr (kSums) {
-            // four groups at a time
-            constexpr int KG = 4 / PG, B = 4;
-            const int count = n * PG;
-            for (int i0 = wave; i0 < count; i0 += B * kWaves) {
-                f32x4 X[B][CT];
-#pragma unroll
-                for (int j = 0; j < B; ++j)
-#pragma unroll
-                    for (int c = 0; c < CT; ++c) X[j][c] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int k0 = 0; k0 < KG; ++k0)
-#pragma unroll
-                    for (int j = 0; j < B; ++j) {
-                        const int i = min(i0 + j * kWaves, count - 1), g = i & (PG - 1);
-                        const uint32_t one = 0x3F803F80u;
-#pragma unroll
-                        for (int c = 0; c < CT; ++c)
-                            X[j][c] = mfma(x_of(i / PG, g * KG + k0, c), u32x4{one, one, one, one}, X[j][c]);
-                    }
-#pragma unroll
-                for (int j = 0; j < B; ++j) {
-                    const int i = min(i0 + j * kWaves, count - 1);
-                    if (r == 0)
-#pragma unroll
-                        for (int c = 0; c < CT; ++c) *reinterpret_cast<f32x4*>(lX + (i * CT + c) * 16 + q * 4) = X[j][c];
-                }
-            }
-            __syncthreads();
-        }
     };
 
     {
@@ -325,17 +291,15 @@ __global__ __launch_bounds__(kWaves * 64, CT == 4 ? 2 : 4) void proj4_kernel(Pro
                     const uint32_t one = 0x3F803F80u;
 #pragma unroll
                     for (int c = 0; c < CT; ++c) {
-                        if constexpr (!kSums) X1[c] = mfma(xf[k % PRE][c], u32x4{one, one, one, one}, X1[c]);
+                        X1[c] = mfma(xf[k % PRE][c], u32x4{one, one, one, one}, X1[c]);
                         D[c] = mfma(xf[k % PRE][c], wf, D[c]);
                     }
                 }
 #pragma unroll
                 for (int c = 0; c < CT; ++c) {
-                    f32x4 X = X1[c];
-                    if constexpr (kSums) X = *reinterpret_cast<const f32x4*>(lX + ((b * PG + g) * CT + c) * 16 + q * 4);
 #pragma unroll
                     for (int m = 0; m < 4; ++m)
-                        acc[c][m] = __builtin_fmaf(s, __builtin_fmaf(-__builtin_fabsf(z), X[m], D[c][m]), acc[c][m]);
+                        acc[c][m] = __builtin_fmaf(s, __builtin_fmaf(-__builtin_fabsf(z), X1[c][m], D[c][m]), acc[c][m]);
                 }
             }
         }
@@ -466,22 +430,24 @@ hipError_t proj4_go(hipStream_t st, Proj4Dev& p) {
     p.nb = (a.K + kBlk - 1) / kBlk;
     p.tiles = (p.half + (a.glu ? 7 : 15)) / (a.glu ? 8 : 16);
     const auto up = [](int n, int d) { return (n + d - 1) / d; };
-    const int x_blk = kChunks * (p.tile_rows * L + 1) * 16, X_blk = GS == 0 || CT <= 2 ? 0 : PG * CT * 64;
+    const int x_blk = kChunks * (p.tile_rows * L + 1) * 16;
     const int s_all = kWaves * kSeg * PG * 16 * (GS == 0 ? 4 : 8), red_most = kWaves * CT * TR * 64;
     // blocks whose x fits beside a second work-group
-    const int fit = std::max(1, int(kLdsHalf - s_all - red_most) / (x_blk + X_blk));
-    // Tiles are shared out over K until there are 8 waves a CU: by waves of a
-    // work-group where all of x fits; where it does not by work-groups, each with
-    // its part of x, and a second launch that sums
-    const int64_t n = int64_t(p.tiles) * p.col_tiles, most = kCus * 8;
-    const int parts = up(p.nb, fit);
+    const int fit = std::max(1, int(kLdsHalf - s_all - red_most) / x_blk);
+    // Tiles are shared out over K, until 4096 waves have one.  Where x would come
+    // to the LDS in three turns or more, by work-groups, each with its part of x,
+    // and a second launch that sums (4 fp32 rows, 7168 x 16384, 3 turns: 23.7 us in
+    // 4 parts, 25.7 by waves; 16 of 2048 x 8192, 2 turns: 12.5 in 4 parts, 9.6 by
+    // waves).  More than 8 parts are slower again (16 rows, 7168 x 4096: 14.5 us in
+    // 4, 12.1 in 8, 16.7 in 16).
+    const int64_t n = int64_t(p.tiles) * p.col_tiles;
     int kw = 1, lks = 0;
-    if (parts > 1) {
-        kw = int(std::max<int64_t>(1, std::min<int64_t>({most / n, int64_t(p.nb), 16})));
-        // few rows: their sums cost less than to go over x in turns
-        if (kw < parts && parts <= 16 && int64_t(parts) * a.T * 64 <= a.K && n * parts <= 2 * most) kw = parts;
-    }
-    while (lks < 3 && (2 << lks) * kw <= p.nb && (n << (lks + 1)) * kw <= most) ++lks;
+    if (p.nb > 2 * fit) kw = int(std::max<int64_t>(1, std::min<int64_t>({kProj4Tiles / n, p.nb / kSeg, 8})));
+    // By waves of a work-group: past 2048 waves only where each keeps two items
+    // (7168 x 32768, one row: 38.5 us by one wave a tile, 31.3 by two; 2048 x 7168:
+    // 6.4 by four, 7.7 by eight with two blocks each).
+    const auto wide = [&](int to) { return (int64_t(2) << to) * kw; };
+    while (lks < 3 && wide(lks) <= p.nb && n * wide(lks) <= (wide(lks) * 2 * kSeg <= p.nb ? kProj4Tiles : kProj4Tiles / 2)) ++lks;
     p.ks = lks;
     const int ks = 1 << p.ks;
     p.sets = up(p.tiles, kWaves / ks);
@@ -493,8 +459,7 @@ hipError_t proj4_go(hipStream_t st, Proj4Dev& p) {
     const int red = ks > 1 ? red_most : 0;
     p.slab = up(p.kw_blocks, up(p.kw_blocks, fit));
     p.wave_blocks = up(p.slab, ks);
-    p.X_at = p.slab * x_blk;
-    p.s_at = p.X_at + p.slab * X_blk;
+    p.s_at = p.slab * x_blk;
     p.red_at = p.s_at + s_all;
     const size_t lds = p.red_at + red;
     if (lds > kLdsMost) return hipErrorInvalidValue;
@@ -512,8 +477,7 @@ hipError_t proj4_x(hipStream_t st, const Proj4Args& a) {
     p.a = a;
     constexpr int TR = XB ? 16 : 4;
     if (a.T <= TR) return proj4_go<GS, XB, 1>(st, p);
-    if (a.T <= 2 * TR) return proj4_go<GS, XB, 2>(st, p);
-    return proj4_go<GS, XB, 4>(st, p);
+    return proj4_go<GS, XB, 2>(st, p);
 }
 
 }  // namespace
