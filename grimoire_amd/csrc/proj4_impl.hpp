@@ -432,7 +432,7 @@ hipError_t proj4_go(hipStream_t st, Proj4Dev& p) {
     const auto up = [](int n, int d) { return (n + d - 1) / d; };
     const int x_blk = kChunks * (p.tile_rows * L + 1) * 16;
     const int s_all = kWaves * kSeg * PG * 16 * (GS == 0 ? 4 : 8), red_most = kWaves * CT * TR * 64;
-    // blocks whose x fits beside a second work-group
+    // blocks whose x fits beside a second work-group (room: with the sums there are)
     const int fit = std::max(1, int(kLdsHalf - s_all - red_most) / x_blk);
     // Tiles are shared out over K, until 4096 waves have one.  Where x would come
     // to the LDS in three turns or more, by work-groups, each with its part of x,
@@ -457,7 +457,8 @@ hipError_t proj4_go(hipStream_t st, Proj4Dev& p) {
     p.kw = up(p.nb, p.kw_blocks);
     if (p.kw > 1 && n * p.kw > kProj4Tiles) return hipErrorInvalidValue;
     const int red = ks > 1 ? red_most : 0;
-    p.slab = up(p.kw_blocks, up(p.kw_blocks, fit));
+    const int room = std::max(1, int(kLdsHalf - s_all - red) / x_blk);
+    p.slab = up(p.kw_blocks, up(p.kw_blocks, room));
     p.wave_blocks = up(p.slab, ks);
     p.s_at = p.slab * x_blk;
     p.red_at = p.s_at + s_all;
