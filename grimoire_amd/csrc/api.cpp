@@ -387,6 +387,7 @@ int grimoire_moe_router_scores_grad(void* stream, const grim_score_params* p, co
         return fail(GRIM_ERR_SHAPE, "n_experts=%d (1..%d)", n_experts, kScoresMaxE);
     if (top_k <= 0 || top_k > kScoresMaxK || top_k > n_experts)
         return fail(GRIM_ERR_SHAPE, "top_k=%d (1..%d)", top_k, kScoresMaxK);
+    if (tokens > kScoresGradMaxTokens) return fail(GRIM_ERR_SHAPE, "tokens=%d (<= %d)", tokens, kScoresGradMaxTokens);
     if (!stride_ok(row_stride, n_experts, 1) || !stride_ok(d_stride, n_experts, 1))
         return fail(GRIM_ERR_SHAPE, "row_stride=%lld d_stride=%lld", (long long)row_stride,
                     (long long)d_stride);
@@ -648,7 +649,7 @@ int grimoire_moe_block_norm(void* stream, const grim_block_norm_params* p, const
 static int route_shape(int tokens, int top_k, int hidden) {
     if (top_k <= 0 || top_k > 16) return fail(GRIM_ERR_SHAPE, "top_k=%d (1..16)", top_k);
     if (hidden <= 0 || hidden % 4) return fail(GRIM_ERR_SHAPE, "hidden=%d (need %% 4)", hidden);
-    if (int64_t(tokens) * top_k > 0x7FFFFFFF) return fail(GRIM_ERR_SHAPE, "tokens * top_k above 2^31 - 1");
+    if (tokens > kSortMaxTokens) return fail(GRIM_ERR_SHAPE, "tokens=%d (<= %d)", tokens, kSortMaxTokens);
     return GRIM_OK;
 }
 

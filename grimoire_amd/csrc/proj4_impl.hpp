@@ -1,4 +1,16 @@
 // proj4_impl.hpp -- the kernel of the dense 4-bit projections (proj4.hip).
+//
+// A wave takes tiles of 16 weight rows (8 gate rows and their up rows) and a
+// part of K, in blocks of 128: 16 bytes a lane, straight to registers, four
+// blocks in flight (through the LDS, with whole lines a wave, was no faster).
+// The words of a lane are one matrix step's operand each; groups of 64
+// and 32 exchange them between lanes so that a step has one group a column.  x
+// lies in the LDS, in operand order, for all of the work-group's tiles; its
+// scales a wave takes through its own part of the LDS, where a load a lane
+// becomes a value a column.  A kernel with many more tiles than work-groups
+// keeps x and goes on with the next weights, whose loads are on their way
+// by then.  Two column tiles of x a work-group at most: four needed 230
+// registers, and 64 rows of 4096 x 8192 took 30.8 us where twos take 21.7.
 #pragma once
 
 #include "proj4_out.hpp"

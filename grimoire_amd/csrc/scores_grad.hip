@@ -10,7 +10,14 @@
 // The choice, and with it a selection bias and groups, has no gradient.  An
 // expert picked twice gets the sum, picks in order.  An expert that is out
 // (logit NaN or -inf) has score and gradient 0; +inf counts as the largest
-// finite logit, as in the scores.
+// finite logit, as in the scores.  All is fp32; an exponential is off by 2 ulp.
+//
+// Bound by the launch at a step's sizes (4096 x 128 fp32, 4 MB: 2 us at a copy's
+// rate, 7.8 a call of which the host takes 5.6).  A wave holds a token's logits in
+// registers, 1 to 8 a lane as E needs, so that each is read once and every sum
+// is one of lanes; the picks lie one a lane.  Renormalised softmax reads the
+// picks' logits alone.  The picks' values go to their experts' places through a
+// row of the LDS, which no other wave reads: no barrier of the work-group.
 #include "scores_grad.hpp"
 
 #include "scores.hpp"

@@ -17,6 +17,8 @@ struct ScoresGradArgs {
     float scaling;
 };
 
+constexpr int kScoresGradMaxTokens = 1 << 24;   // a wavefront a token, 2^32 threads a launch
+
 hipError_t scores_grad_launch(hipStream_t st, const ScoresGradArgs& a);
 
 }  // namespace grim

@@ -4,6 +4,14 @@
 //   sort_grad     dx[t] = sum_s w[t,s] drows[p],        dw[t,s] = <drows[p], x[t]>
 //   combine_grad  drows[p] = w[t,s] dy[t],              dw[t,s] = <dy[t], rows[p]>,
 //                 dshared[t] = gate[t] dy[t],           dgate[t] = <dy[t], shared[t]>
+// All are bound by the memory: each row is read or written once, past the
+// caches (a batch's rows are larger than they, and 4096 x 10 rows of 2048 bf16
+// took 5 - 40 % longer through them).  A token's work-group has its element of
+// x or dy in registers for all of its slots, and unrolled for their number,
+// so that the slots' rows are asked for together (a loop with an exit in it
+// took 10 us more at 4096 x 10).  Products are fp32, rounded once to bf16;
+// dots are an fp32 chain a thread, then lanes, then waves in order: the same
+// bits every time.
 #include "sort_rows.hpp"
 
 #include "dispatch.hpp"
@@ -14,6 +22,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kMaxSlots = 16;
+constexpr int kCus = 256;
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
@@ -150,11 +159,12 @@ __device__ __forceinline__ void count_experts(const SortRowsArgs& a, int32_t* hi
     }
 }
 
-// The whole sort of a batch of at most kBruteRoutes routes in one launch: a
+// Small batches.  The whole sort of at most kBruteRoutes routes in one launch: a
 // work-group takes a token and counts, for each of its routes, the routes
 // before it in expert order (keys expert * 2^13 + route, each lane a share of
 // them).  One more work-group writes the experts' counts and offsets.
-// blockIdx.y: part of the columns.
+// blockIdx.y: part of the columns.  What it costs is the chain of its waits (the
+// ids, a barrier, x) and of a launch: 2 tokens x 8 4.7 us, 64 x 8 of 2048 5.2 us.
 constexpr int kBruteRoutes = 8192, kBruteE = 2048;
 constexpr uint32_t kNoKey = 0xFFFFFFFFu;
 template <bool XB, bool RB, int KT, int V>
@@ -213,7 +223,11 @@ __global__ __launch_bounds__(kThreads) void sort_brute_kernel(SortRowsArgs a, in
 // The table of a batch of at most kTableRoutes routes in one launch: each
 // work-group counts all routes by expert, those before its own apart, and
 // ranks its own kThreads routes behind them.  No counts pass through memory;
-// what each reads again, the ids, lies in the L2.
+// what each reads again, the ids, lies in the L2: 4096 x 10 routes over 512
+// experts with their rows of 2048 bf16 take 43.1 us (rows written at 4.9 TB/s),
+// with the four launches of dispatch.hip 51.0; 2048 x 8 of 1024 15.9 and 23.3.
+// Past 65536 routes reading them 256 times costs more than those (72000: 56.2 us
+// and 53.7).
 constexpr int kTableRoutes = 65536, kTableThreads = 1024;
 __global__ __launch_bounds__(kTableThreads) void sort_table_kernel(SortRowsArgs a) {
     __shared__ int32_t before[kBruteE], behind[kBruteE];   // routes of an expert before the block, and from it on
@@ -296,6 +310,8 @@ __global__ __launch_bounds__(kThreads) void sort_rows_kernel(SortRowsArgs a) {
     copy_rows<XB, RB, KT, V>(a, t, p, 0, a.H);
 }
 
+// dx and the weights' gradients: a work-group a token.  3001 x 4 rows of 2880
+// bf16: 4.6 TB/s; 4096 x 10 of 2048 with weights 42.5 us, 4.7 TB/s.
 template <bool RB, bool XB, int KT, int V>
 __global__ __launch_bounds__(1024) void sort_grad_kernel(SortGradArgs a) {
     __shared__ float part[1024 / kWave * KT];
@@ -337,7 +353,9 @@ __global__ __launch_bounds__(1024) void sort_grad_kernel(SortGradArgs a) {
     }
 }
 
-// slots blockIdx.y * KT ...; the first of them does the shared expert too
+// The gradient of the combine, a work-group a token and KT slots, blockIdx.y *
+// KT ...; the first of them does the shared expert too.  Reads and writes as
+// many rows: 4096 x 10 of 2048 bf16 79 us, 4.9 TB/s, what a copy reaches.
 template <bool YB, bool RB, int KT, int V>
 __global__ __launch_bounds__(KT == 1 ? 1024 : kThreads) void combine_grad_kernel(CombineGradArgs a) {
     __shared__ float part[(KT == 1 ? 1024 : kThreads) / kWave * (KT + 1)];
@@ -402,10 +420,11 @@ hipError_t sort_k(hipStream_t st, const SortRowsArgs& a) {
     const int64_t R = int64_t(a.T) * a.K;
     // One launch while the counting costs less than a second launch: every
     // token's work-group reads all routes, (8 + 3 KT) / 64 operations a route
-    // (64 tokens x 8: 6 us where a table and the rows take 9; 1024 x 8 even;
-    // 4096 x 2: 60 against 52)
+    // (rows of 2048 bf16, one launch and two: 64 tokens x 8 5.2 and 9.2 us, 512 x 8
+    // 10.5 and 11.5; 1024 x 8 23.8 and 15.3, 4096 x 2 31 and 16)
     if (R <= kBruteRoutes && a.E <= kBruteE && R * a.T * (8 + 3 * KT) <= 100'000'000) {
-        // columns shared out until there are some work-groups a CU
+        // columns shared out until there are two work-groups a CU (8 tokens x 8
+        // of 7168: 4.8 us, undivided 9.9; 64: 6.6 and 10.7)
         const int most = (a.H + kThreads * V - 1) / (kThreads * V);
         const int parts = a.T >= 512 ? 1 : most < 512 / a.T ? most : 512 / a.T;
         const int cols = ((a.H + parts - 1) / parts + V - 1) / V * V;
@@ -449,6 +468,8 @@ hipError_t sort_rows_launch(hipStream_t st, const SortRowsArgs& a) {
         return hipGetLastError();
     }
     if (a.K <= 0 || a.K > kMaxSlots || a.H % 4) return hipErrorInvalidValue;
+    // 16 bytes of a bf16 row a lane where they are aligned (4096 x 10 of 2048: 42.6
+    // us, by 8 bytes 46.0); of an fp32 row too, so that a wave's are side by side
     const bool v8 = a.H % 8 == 0 && by8(a.x, a.x_stride, a.x_bf16) && by8(a.rows, a.H, a.rows_bf16);
 #define GRIM_SORT(XB, RB) RB && v8 ? sort_slots<XB, RB, RB ? 8 : 4>(st, a) : sort_slots<XB, RB, 4>(st, a)
     if (a.x_bf16) return a.rows_bf16 ? (GRIM_SORT(true, true)) : (GRIM_SORT(true, false));
@@ -460,7 +481,9 @@ namespace {
 
 template <bool RB, bool XB, int V>
 void sort_grad_k(hipStream_t st, const SortGradArgs& a) {
-    const int threads = a.T < 256 && a.H > kThreads * V ? 1024 : kThreads;
+    // less than a work-group a CU: larger ones (8 slots of 7168: 32 tokens 11.5 ->
+    // 8.0 us, 255 15.1 -> 11.8; 512 21.1 -> 22.4)
+    const int threads = a.T < kCus && a.H > kThreads * V ? 1024 : kThreads;
 #define GRIM_GRAD(KT) hipLaunchKernelGGL((sort_grad_kernel<RB, XB, KT, V>), dim3(a.T), dim3(threads), 0, st, a)
     if (a.K <= 1) GRIM_GRAD(1);
     else if (a.K <= 2) GRIM_GRAD(2);
@@ -474,8 +497,10 @@ void sort_grad_k(hipStream_t st, const SortGradArgs& a) {
 
 template <bool YB, bool RB, int V>
 void combine_grad_k(hipStream_t st, const CombineGradArgs& a) {
-    // few tokens: a work-group a slot, of as many threads as a row has pieces
-    const bool few = a.T <= 64;
+    // Few tokens: a larger work-group a slot, which reads dy again (8 slots of 7168:
+    // 32 tokens 20.4 -> 5.7 us, 256 24.8 -> 20.7, 1024 61 -> 74; 4 of 2880: 256 8.3
+    // and 8.3, 512 12.3 -> 14.1).
+    const bool few = a.T <= kCus;
     const int threads = few && a.H > kThreads * V ? 1024 : kThreads;
 #define GRIM_GRAD(KT) \
     hipLaunchKernelGGL((combine_grad_kernel<YB, RB, KT, V>), dim3(a.T, (a.K + KT - 1) / KT), dim3(threads), 0, st, a)

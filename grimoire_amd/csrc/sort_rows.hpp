@@ -52,6 +52,7 @@ struct CombineGradArgs {
     int T, K, H;
 };
 
+constexpr int kSortMaxTokens = 1 << 23;   // a work-group a token, 2^32 threads a launch
 constexpr int kSortMaxE = 16384;     // a count a byte quad in 64 KiB of LDS
 
 size_t sort_rows_workspace_bytes(int T, int K, int E);

@@ -218,7 +218,8 @@ int grimoire_moe_router_scores(void* stream, const grim_score_params* p, const v
  * expert picked twice gets the sum.  An expert whose logit is NaN or -inf has
  * score and gradient 0; +inf counts as the largest finite logit.  dlogits:
  * rows of the logits' type, d_stride elements apart, every element written;
- * it may be the logits themselves (same stride).  Sums are fp32. */
+ * it may be the logits themselves (same stride).  Sums are fp32.  Up to 2^24
+ * tokens. */
 int grimoire_moe_router_scores_grad(void* stream, const grim_score_params* p, const void* logits,
                                     int logits_bf16, int64_t row_stride, const int32_t* expert,
                                     const float* dweight, void* dlogits, int64_t d_stride, int tokens,
@@ -369,10 +370,10 @@ int grimoire_moe_combine(void* stream, const uint16_t* src, const int32_t* inver
  * A route whose expert is outside [0, num_experts), or whose inverse is outside
  * [0, n_rows), has no row: it adds nothing, its dweight is 0.  Rows that no
  * route names keep what drows holds; the routes of one call name different
- * rows (of several routes to one row, one writes it).  x, dx and dy: fp32 or
+ * rows (of several to one row, any of them writes each element).  x, dx and dy: fp32 or
  * bf16, rows an own distance of elements apart (a multiple of 4, <= 2^28); the other
  * rows lie one behind the other.  drows has the rows' type, dshared shared's.
- * Sums are fp32, rounded once.  hidden % 4 == 0, top_k <= 16; fp32 rows
+ * Sums are fp32, rounded once.  hidden % 4 == 0, top_k <= 16, up to 2^23 tokens; fp32 rows
  * 16-byte, bf16 rows 8-byte aligned (with 16 bytes and hidden and distances a
  * multiple of 8, bf16 is accessed 16 bytes at a time).  No output overlaps
  * another argument.  sort_rows takes a workspace (4-byte aligned, no initial

@@ -214,6 +214,19 @@ def test_zero_and_extreme_scales(gpu):
     assert torch.isnan(y[:, 2]).all()
 
 
+@pytest.mark.parametrize("code", [0, 1])
+def test_smallest_scales(gpu, code):
+    """MXFP4's scales of 2^-127 and 2^-126: weights below bf16's and fp32's normal
+    numbers, large rows."""
+    m = make_weight("mxfp4", "none", 16, 64, 32, 4)
+    for x_bf16 in (False, True):
+        x = rows(3, 64, 6, x_bf16) * 1e30
+        m.scales[:] = code + 100
+        v, tol = reference(m, x)
+        m.scales[:] = code
+        check(run(gpu, m, x), v * 2.0 ** -100, tol * 2.0 ** -100)
+
+
 def test_no_rows(gpu):
     w = make_weight("int4", "asym", 16, 64, 32, 1)
     proj = ops.Projection4(w.to(gpu), 4)

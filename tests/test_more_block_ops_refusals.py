@@ -146,3 +146,9 @@ def test_scores_grad_arguments(kw, status):
 
 def test_no_tokens():
     assert scores(T=0, l=None) == 0 and combine(T=0, dy=None) == 0 and sort_grad(T=0, dx=None) == 0
+
+
+def test_more_tokens_than_a_launch_takes():
+    n = (1 << 23) + 1
+    assert sort(T=n, K=1, n=1 << 62) == SHAPE and sort_grad(T=n, K=1) == SHAPE and combine(T=n, K=1) == SHAPE
+    assert scores(T=(1 << 24) + 1) == SHAPE
