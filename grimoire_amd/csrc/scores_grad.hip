@@ -61,6 +61,13 @@ __global__ __launch_bounds__(kWaves * kWave) void scores_grad_kernel(ScoresGradA
     const float ninf = -__builtin_inff();
     const bool full = !a.sigmoid && !a.normalize;    // the softmax over all experts counts
     float* mine = row[wave];
+    float lv[NV];
+    if (full)                                        // on their way while the picks are read
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int e = j * kWave + lane;
+            lv[j] = logit<BF16>(a.logits, t * a.row_stride + (e < E ? e : E - 1));
+        }
 #pragma unroll
     for (int j = 0; j < NV; ++j) mine[j * kWave + lane] = 0.0f;
 
@@ -70,13 +77,12 @@ __global__ __launch_bounds__(kWaves * kWave) void scores_grad_kernel(ScoresGradA
     const float pl = id >= 0 ? logit<BF16>(a.logits, t * a.row_stride + id) : ninf;
     const float g = id >= 0 ? a.dw[t * a.K + lane] * a.scaling : 0.0f;
 
-    float lv[NV], m = 0.0f, iz = 0.0f, u, sum = 0.0f, d;
+    float m = 0.0f, iz = 0.0f, u, sum = 0.0f, d;
     if (full) {
         float top = ninf;
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-            const int e = j * kWave + lane;
-            lv[j] = e < E ? logit<BF16>(a.logits, t * a.row_stride + e) : ninf;
+            lv[j] = j * kWave + lane < E ? lv[j] : ninf;
             top = fmaxf(top, lv[j]);
         }
         top = wave_max(top);

@@ -249,18 +249,21 @@ __global__ __launch_bounds__(kTableThreads) void sort_table_kernel(SortRowsArgs 
         for (int j = 0; j < B; ++j) e[j] = a.ids[min(r + j * kTableThreads, R - 1)];
 #pragma unroll
         for (int j = 0; j < B; ++j) {
-            const int at = r + j * kTableThreads;
-            if (at < R && e[j] >= 0 && e[j] < E) atomicAdd(at < r0 ? &before[e[j]] : &behind[e[j]], 1);
+            const int at = r + j * kTableThreads;      // a wave's are all before the block or all behind
+            int32_t* to = __builtin_amdgcn_readfirstlane(at) < r0 ? before : behind;
+            if (at < R && uint32_t(e[j]) < uint32_t(E)) atomicAdd(&to[e[j]], 1);
         }
     }
     // earlier routes of the block's with the same expert, a quarter of them each
     int n = 0;
     constexpr int Q = kThreads / (kTableThreads / kThreads);
+    static_assert(Q == kWave, "a wave's routes are one quarter");
+    if (part <= __builtin_amdgcn_readfirstlane(i) / Q)
 #pragma unroll 4
-    for (int j = part * Q; j < (part + 1) * Q; j += 4) {
-        const int4 e = *reinterpret_cast<const int4*>(&le[j]);
-        n += (j < i && e.x == my) + (j + 1 < i && e.y == my) + (j + 2 < i && e.z == my) + (j + 3 < i && e.w == my);
-    }
+        for (int j = part * Q; j < (part + 1) * Q; j += 4) {
+            const int4 e = *reinterpret_cast<const int4*>(&le[j]);
+            n += (j < i && e.x == my) + (j + 1 < i && e.y == my) + (j + 2 < i && e.z == my) + (j + 3 < i && e.w == my);
+        }
     rank[part][i] = n;
     __syncthreads();
     // exclusive offsets of the experts: this thread's are [e0, e1)
