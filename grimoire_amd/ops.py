@@ -646,7 +646,7 @@ class Projection4:
             raise _abi.GrimoireError(f"weight format {weight.fmt}: INT4, INT4_F16 or MXFP4")
         if weight.payload.dim() != 2 or weight.scales is None:
             raise _abi.GrimoireError("weight: payload [N][bytes of a row] and scales")
-        bits = (torch.uint8,) if weight.fmt == _abi.FMT_MXFP4 else (_i16, _b16, torch.float16)
+        bits = {_abi.FMT_MXFP4: (torch.uint8,), _abi.FMT_INT4: _B16, _abi.FMT_INT4_F16: (torch.float16, _i16)}[weight.fmt]
         _flat(weight.payload, "payload", (N, weight.row_bytes), (torch.uint8,), self.dev)
         _flat(weight.scales, "scales", (N, g), bits, self.dev)
         _flat(weight.zeros, "zeros", (N, g), (torch.uint8,), self.dev)

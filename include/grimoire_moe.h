@@ -534,7 +534,7 @@ int grimoire_lora_swiglu(void* stream, const grim_lora* L, const int32_t* row_sl
  * may lie beside each other in one buffer.  Codes and fp32 or bf16 activations
  * are multiplied exactly, sums are fp32.  A row of x with an infinity or a NaN
  * gives NaN or infinities in its own row alone; finite x should stay below
- * 1e36 (codes are multiplied as 16 + q).  Up to 2^19 rows; the weights are
+ * 5e33 (codes are multiplied as 16 + q).  Up to 2^18 rows; the weights are
  * read again for every 32 (bf16) or 8 (fp32) of them.
  * The workspace holds grimoire_proj4_workspace_bytes for up to `rows` rows
  * (16-byte aligned, no initial contents, apart from every other argument);

@@ -195,6 +195,31 @@ def test_row_that_is_not_finite(gpu, fmt, zeros, x_bf16):
     assert not torch.isfinite(y[3].cpu()[hit]).any()
 
 
+@pytest.mark.parametrize("x_bf16", [False, True])
+def test_large_rows(gpu, x_bf16):
+    """Rows up to 5e33 with the zero points farthest from the codes: (16 + q + 16 + z)
+    times a group's sum stays a number."""
+    w = make_weight("int4", "mixed", 64, 512, 128, 4)
+    x = rows(5, 512, 6, x_bf16).clamp(-4, 4) * 1.2e33
+    check(run(gpu, w, x), *reference(w, x))
+
+
+@pytest.mark.parametrize("x_bf16", [False, True])
+def test_rows_far_apart(gpu, x_bf16):
+    """Rows of x, y and base whose offsets pass 32 bits."""
+    T, K, N, S = 40, 256, 48, 1 << 26
+    w = make_weight("int4", "asym", N, K, 64, 4)
+    x, base = rows(T, K, 6, x_bf16), rows(T, N, 7)
+    xg = torch.empty(((T - 1) * S + K,), device=gpu, dtype=x.dtype).as_strided((T, K), (S, 1))
+    y = torch.empty(((T - 1) * S + N,), device=gpu).as_strided((T, N), (S, 1))
+    bg = torch.empty(((T - 1) * S + N,), device=gpu).as_strided((T, N), (S, 1))
+    assert (T - 1) * S > 2 ** 31
+    xg.copy_(x)
+    bg.copy_(base)
+    ops.Projection4(w.to(gpu), T)(xg, y, base=bg)
+    check(y, *reference(w, x, base))
+
+
 def test_zero_and_extreme_scales(gpu):
     """Scales of 0, the smallest and the largest; MXFP4's 2^-127 and 2^127, and
     its NaN in the rows and groups that have it."""
@@ -324,6 +349,8 @@ def test_host_refusals_on_the_gpu_objects(gpu):
     for bad in (Weight(_abi.FMT_INT8, 16, 64, w.payload, w.scales, None, 1),
                 Weight(w.fmt, 16, 64, w.payload, w.scales.float(), w.zeros, 2),
                 Weight(w.fmt, 16, 64, w.payload, w.scales[:8], w.zeros, 2),
+                Weight(w.fmt, 16, 64, w.payload, w.scales.view(torch.float16), w.zeros, 2),
+                Weight(_abi.FMT_INT4_F16, 16, 64, w.payload, w.scales.view(torch.bfloat16), w.zeros, 2),
                 Weight(w.fmt, 16, 64, w.payload.cpu(), w.scales, w.zeros, 2)):
         with pytest.raises(_abi.GrimoireError):
             ops.Projection4(bad, 4)

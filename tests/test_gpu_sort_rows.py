@@ -365,6 +365,25 @@ def test_offsets_past_32_bits(gpu):
     assert torch.equal(drows[-T:], (x.float() * 0.5).bfloat16()) and torch.equal(dw[:, 0], dw[:, 7])
 
 
+def test_rows_far_apart(gpu):
+    """Rows of x, dx and dy whose offsets pass 32 bits."""
+    T, E, K, H, S = 40, 16, 4, 264, 1 << 26
+    assert (T - 1) * S > 2 ** 31
+    ids = routes(T, E, K, 3)
+    x, w = data(T, H, K, 4)
+    inv = table(ids, E)[0]
+    view, dx = (torch.empty(((T - 1) * S + H,), device=gpu).as_strided((T, H), (S, 1)) for _ in range(2))
+    view.copy_(x)
+    obj = ops.TokenSort(E, K, T, device=gpu)
+    check_sort(sort_view(gpu, obj, ids, view, E, w), ids, x, E, True, w)
+    drows = torch.randn((T * K, H), generator=gen(1))
+    dw = torch.empty((T, K), device=gpu)
+    obj.grad(drows.to(gpu), inv.to(gpu), dx, x=view, weight=w.to(gpu), dweight=dw)
+    torch.cuda.synchronize()
+    check_sort_grad(dx.cpu(), dw.cpu(), drows, inv.view(T, K), x, w)
+    check_combine(gpu, T, K, H, 11, dy=view, dy_cpu=x, inv=inv)
+
+
 def test_host_refusals_on_the_gpu_objects(gpu):
     T, E, K, H = 4, 8, 2, 16
     obj = ops.TokenSort(E, K, T, device=gpu)

@@ -57,6 +57,13 @@ def test_projection_arguments(kw, status):
     assert proj(**kw) == status
 
 
+@pytest.mark.parametrize("w", [dict(K=512, row_bytes=256, row_scales=1), dict(row_scales=0), dict(row_scales=-1),
+                               dict(K=1024, row_bytes=512, row_scales=2)])
+def test_groups_that_there_are_not(w):
+    assert proj(weight(**w), xs=1024) == SHAPE
+    assert glu(weight(**w), xs=1024) == SHAPE
+
+
 def test_projection_no_rows_and_odd_glu():
     assert proj(rows=0, x=None, y=None) == 0
     assert glu(weight(N=63)) == SHAPE
@@ -68,6 +75,11 @@ def test_projection_no_rows_and_odd_glu():
     n = [_abi.lib().grimoire_proj4_workspace_bytes(C.byref(w), r) for r in (-1, 0, 1, 4, 64, 65, 1 << 20)]
     assert n[0] == n[1] == 0 and 0 < n[2] < n[3] < n[4] == n[5] == n[6]
     assert proj(n=n[3], y=None) == ARG and proj(n=n[3] - 1) == WS
+
+
+def test_more_rows_than_a_launch_takes():
+    assert proj(rows=(1 << 18) + 1) == SHAPE and glu(rows=(1 << 18) + 1) == SHAPE
+    assert proj(rows=1 << 18, n=1 << 62, ws=None) == WS
 
 
 def sort(**kw):
