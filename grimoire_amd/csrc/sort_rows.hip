@@ -161,11 +161,11 @@ __device__ __forceinline__ void count_experts(const SortRowsArgs& a, int32_t* hi
 
 // Small batches.  The whole sort of at most kBruteRoutes routes in one launch: a
 // work-group takes a token and counts, for each of its routes, the routes
-// before it in expert order (keys expert * 2^13 + route, each lane a share of
+// before it in expert order (keys expert * 2^12 + route, each lane a share of
 // them).  One more work-group writes the experts' counts and offsets.
 // blockIdx.y: part of the columns.  What it costs is the chain of its waits (the
 // ids, a barrier, x) and of a launch: 2 tokens x 8 4.7 us, 64 x 8 of 2048 5.2 us.
-constexpr int kBruteRoutes = 8192, kBruteE = 2048;
+constexpr int kBruteRoutes = 4096, kBruteE = 2048;
 constexpr uint32_t kNoKey = 0xFFFFFFFFu;
 template <bool XB, bool RB, int KT, int V>
 __global__ __launch_bounds__(kThreads) void sort_brute_kernel(SortRowsArgs a, int cols) {
@@ -179,7 +179,7 @@ __global__ __launch_bounds__(kThreads) void sort_brute_kernel(SortRowsArgs a, in
         return;
     }
     auto key_of = [&](int r, int e) {
-        return r < R && e >= 0 && e < E ? uint32_t(e) << 13 | uint32_t(r) : kNoKey;
+        return r < R && e >= 0 && e < E ? uint32_t(e) << 12 | uint32_t(r) : kNoKey;
     };
     // lane s: this token's route s
     const bool slot = lane < a.K;
@@ -224,23 +224,20 @@ __global__ __launch_bounds__(kThreads) void sort_brute_kernel(SortRowsArgs a, in
 // work-group counts all routes by expert, those before its own apart, and
 // ranks its own kThreads routes behind them.  No counts pass through memory;
 // what each reads again, the ids, lies in the L2: 4096 x 10 routes over 512
-// experts with their rows of 2048 bf16 take 43.1 us (rows written at 4.9 TB/s),
-// with the four launches of dispatch.hip 51.0; 2048 x 8 of 1024 15.9 and 23.3.
-// Past 65536 routes reading them 256 times costs more than those (72000: 56.2 us
-// and 53.7).
-constexpr int kTableRoutes = 65536, kTableThreads = 1024;
+// experts with their rows of 2048 bf16 take 41.4 us (rows written at 5.2 TB/s),
+// with the four launches of dispatch.hip 51; 2048 x 8 of 1024 14.5 and 23.3.
+// Reading them once per 256 costs more than those past about 100000 routes (96000
+// with rows of 1024: 61.8 us and 65.4, 131072 91.2 and 85.1).
+constexpr int kTableRoutes = 98304, kTableThreads = 1024;
 __global__ __launch_bounds__(kTableThreads) void sort_table_kernel(SortRowsArgs a) {
     __shared__ int32_t before[kBruteE], behind[kBruteE];   // routes of an expert before the block, and from it on
-    __shared__ __attribute__((aligned(16))) int32_t le[kThreads];
-    __shared__ int32_t rank[kTableThreads / kThreads][kThreads];
     __shared__ int32_t wsum[kTableThreads / kWave];
     const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
     const int E = a.E, R = a.T * a.K, r0 = blockIdx.x * kThreads;
     for (int e = tid; e < E; e += kTableThreads) before[e] = behind[e] = 0;
-    const int i = tid & (kThreads - 1), part = tid / kThreads;
-    int my = r0 + i < R ? a.ids[r0 + i] : -1;
+    // this thread's route: four waves have one
+    int my = tid < kThreads && r0 + tid < R ? a.ids[r0 + tid] : -1;
     my = my >= 0 && my < E ? my : -1;
-    if (part == 0) le[i] = my;
     __syncthreads();
     constexpr int B = 8;                               // loads in flight
     for (int r = tid; r < R; r += B * kTableThreads) {
@@ -254,17 +251,14 @@ __global__ __launch_bounds__(kTableThreads) void sort_table_kernel(SortRowsArgs 
             if (at < R && uint32_t(e[j]) < uint32_t(E)) atomicAdd(&to[e[j]], 1);
         }
     }
-    // earlier routes of the block's with the same expert, a quarter of them each
-    int n = 0;
-    constexpr int Q = kThreads / (kTableThreads / kThreads);
-    static_assert(Q == kWave, "a wave's routes are one quarter");
-    if (part <= __builtin_amdgcn_readfirstlane(i) / Q)
-#pragma unroll 4
-        for (int j = part * Q; j < (part + 1) * Q; j += 4) {
-            const int4 e = *reinterpret_cast<const int4*>(&le[j]);
-            n += (j < i && e.x == my) + (j + 1 < i && e.y == my) + (j + 2 < i && e.z == my) + (j + 3 < i && e.w == my);
-        }
-    rank[part][i] = n;
+    // the lanes of this wave with the same expert, by the bits of its number
+    uint64_t same = __ballot(my >= 0);
+    for (int b = 0; (E - 1) >> b; ++b) {
+        const bool bit = my >> b & 1;
+        const uint64_t m = __ballot(bit);
+        same &= bit ? m : ~m;
+    }
+    const int rank = __popcll(same & ((uint64_t(1) << lane) - 1)), count = __popcll(same);
     __syncthreads();
     // exclusive offsets of the experts: this thread's are [e0, e1)
     const int pe = (E + kTableThreads - 1) / kTableThreads, e0 = min(tid * pe, E), e1 = min(e0 + pe, E);
@@ -290,16 +284,19 @@ __global__ __launch_bounds__(kTableThreads) void sort_table_kernel(SortRowsArgs 
         before[e] += base;                             // the row of the block's first route of e
         base += c;
     }
-    __syncthreads();
-    if (part == 0 && r0 + i < R) {
-        int row = -1;
-        if (my >= 0) {
-            row = before[my];
-#pragma unroll
-            for (int q = 0; q < kTableThreads / kThreads; ++q) row += rank[q][i];
-            if (a.perm_token) a.perm_token[row] = (r0 + i) / a.K;
+    // the block's waves in turn, each moving its experts' rows on
+    int row = -1;
+    for (int w = 0; w < kThreads / kWave; ++w) {
+        __syncthreads();
+        if (wave == w && my >= 0) {
+            const int first = before[my];
+            row = first + rank;
+            if (rank == count - 1) before[my] = first + count;
         }
-        a.inverse[r0 + i] = row;
+    }
+    if (tid < kThreads && r0 + tid < R) {
+        if (row >= 0 && a.perm_token) a.perm_token[row] = (r0 + tid) / a.K;
+        a.inverse[r0 + tid] = row;
     }
 }
 
@@ -423,9 +420,9 @@ hipError_t sort_k(hipStream_t st, const SortRowsArgs& a) {
     const int64_t R = int64_t(a.T) * a.K;
     // One launch while the counting costs less than a second launch: every
     // token's work-group reads all routes, (8 + 3 KT) / 64 operations a route
-    // (rows of 2048 bf16, one launch and two: 64 tokens x 8 5.2 and 9.2 us, 512 x 8
-    // 10.5 and 11.5; 1024 x 8 23.8 and 15.3, 4096 x 2 31 and 16)
-    if (R <= kBruteRoutes && a.E <= kBruteE && R * a.T * (8 + 3 * KT) <= 100'000'000) {
+    // (rows of 2048 bf16, one launch and two: 64 tokens x 8 5.3 and 8.0 us, 400 x 8
+    // 9.5 and 10.0, 2000 x 1 7.9 and 9.0; 512 x 8 10.4 and 10.2, 300 x 10 12.9 and 11.2)
+    if (R <= kBruteRoutes && a.E <= kBruteE && R * a.T * (8 + 3 * KT) <= 45'000'000) {
         // columns shared out until there are two work-groups a CU (8 tokens x 8
         // of 7168: 4.8 us, undivided 9.9; 64: 6.6 and 10.7)
         const int most = (a.H + kThreads * V - 1) / (kThreads * V);

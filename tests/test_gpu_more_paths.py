@@ -16,6 +16,8 @@ pytestmark = pytest.mark.gpu
     (512, 2048, 16, 8), (512, 2049, 16, 8),        # 2048 experts
     (1170, 64, 7, 20), (8192, 40, 1, 4), (4096, 2048, 2, 4), (4097, 2048, 2, 4),
     (8192, 100, 8, 4), (8193, 100, 8, 4),          # 65536 routes
+    (12288, 100, 8, 4), (12289, 100, 8, 4),        # 98304
+    (418, 30, 8, 8), (420, 30, 8, 8), (223, 30, 16, 8), (225, 30, 16, 8), (2022, 30, 1, 8), (2023, 30, 1, 8),
     (65536, 7, 1, 4), (65537, 7, 1, 4), (9001, 2048, 16, 4)])
 def test_sort_sizes(gpu, T, E, K, H):
     for n, kind in enumerate(("mixed", "one")):
