@@ -38,19 +38,17 @@ __global__ __launch_bounds__(256) void proj4_sum_kernel(Proj4Dev p) {
     const int64_t step = int64_t(a.T) * p.tiles * 16;
     const int gu = a.glu ? 8 : 0;
     float o = 0.0f, up = 0.0f;
-    for (int k0 = 0; k0 < p.kw; k0 += 4) {             // four parts at a time (a missing one is not used)
-        float e[4], f[4];
+    float e[kProj4Parts], f[kProj4Parts];              // all asked for together (a missing one is not used)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const float* from = at + (k0 + k < p.kw ? k0 + k : 0) * step;
-            e[k] = from[0];
-            f[k] = from[gu];
-        }
+    for (int k = 0; k < kProj4Parts; ++k) {
+        const float* from = at + (k < p.kw ? k : 0) * step;
+        e[k] = from[0];
+        f[k] = from[gu];
+    }
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            o += k0 + k < p.kw ? e[k] : 0.0f;
-            up += k0 + k < p.kw ? f[k] : 0.0f;
-        }
+    for (int k = 0; k < kProj4Parts; ++k) {
+        o += k < p.kw ? e[k] : 0.0f;
+        up += k < p.kw ? f[k] : 0.0f;
     }
     proj4_out(a, t, n, o, up);
 }

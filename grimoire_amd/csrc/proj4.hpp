@@ -34,9 +34,9 @@ struct Proj4Dev {
 };
 
 constexpr int kProj4MaxRows = 1 << 18;     // parts of 8 rows, 65535 of which a grid takes
-// Sums over parts of K are of at most this many (tile of 16 outputs, part of K,
+// Sums over at most kProj4Parts parts of K are of at most this many (tile of 16 outputs, part of K,
 // work-group's rows of x), whose rows are at most kProj4TileRows.
-constexpr int kProj4Tiles = 4096, kProj4TileRows = 32;
+constexpr int kProj4Tiles = 4096, kProj4TileRows = 32, kProj4Parts = 8;
 inline size_t proj4_workspace_bytes(int rows) {
     return size_t(kProj4Tiles) * 64 * (rows < kProj4TileRows ? rows : kProj4TileRows);
 }

@@ -454,7 +454,7 @@ hipError_t proj4_go(hipStream_t st, Proj4Dev& p) {
     // 4, 12.1 in 8, 16.7 in 16).
     const int64_t n = int64_t(p.tiles) * p.col_tiles;
     int kw = 1, lks = 0;
-    if (p.nb > 2 * fit) kw = int(std::max<int64_t>(1, std::min<int64_t>({kProj4Tiles / n, p.nb / kSeg, 8})));
+    if (p.nb > 2 * fit) kw = int(std::max<int64_t>(1, std::min<int64_t>({kProj4Tiles / n, p.nb / kSeg, kProj4Parts})));
     // By waves of a work-group: past 2048 waves only where each keeps two items
     // (7168 x 32768, one row: 38.5 us by one wave a tile, 31.3 by two; 2048 x 7168:
     // 6.4 by four, 7.7 by eight with two blocks each).
