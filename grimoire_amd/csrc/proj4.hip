@@ -15,9 +15,9 @@
 // conversion instruction gives w s in bf16, exact.  Sums are fp32.
 //
 // What bounds it now (kernel alone, weights in no cache): one row of 7168 x
-// 32768 INT4 31 us, 4.0 TB/s, 78 % of a copy's rate; the decoding
-// (51 to 84 vector operations for 1 KiB of codes and 64 lanes) and the
-// loads in flight share what is missing.  Small ones are chains: 768 x 2048 5.2
+// 32768 INT4 31 us, 4.0 TB/s, 78 % of a copy's rate; its loads alone take 30, the
+// decoding alone (51 to 84 vector operations for 1 KiB of codes and 64 lanes) 23,
+// x and the launch 4 of either.  Small ones are chains: 768 x 2048 5.2
 // us, 2880 x 5760 with SwiGLU for 8 rows 8.2 (fetch x, LDS, the first weights, the
 // sum over the waves).  32 rows of 7168 x 4096 with SwiGLU 16.1 us: 58 KB of x a
 // part of K in each work-group, and the second launch that sums.

@@ -310,10 +310,11 @@ __global__ __launch_bounds__(kThreads) void sort_rows_kernel(SortRowsArgs a) {
     copy_rows<XB, RB, KT, V>(a, t, p, 0, a.H);
 }
 
-// dx and the weights' gradients: a work-group a token.  3001 x 4 rows of 2880
+// dx and the weights' gradients: a work-group a token, or without the weights'
+// a token's columns blockIdx.y * cols ....  3001 x 4 rows of 2880
 // bf16: 4.6 TB/s; 4096 x 10 of 2048 with weights 42.5 us, 4.7 TB/s.
 template <bool RB, bool XB, int KT, int V>
-__global__ __launch_bounds__(1024) void sort_grad_kernel(SortGradArgs a) {
+__global__ __launch_bounds__(1024) void sort_grad_kernel(SortGradArgs a, int cols) {
     __shared__ float part[1024 / kWave * KT];
     const int64_t t = blockIdx.x;
     int64_t p[KT];
@@ -326,7 +327,8 @@ __global__ __launch_bounds__(1024) void sort_grad_kernel(SortGradArgs a) {
         w[s] = a.w ? a.w[at] : 1.0f;
         dot[s] = 0.0f;
     }
-    for (int d = threadIdx.x * V; d < a.H; d += blockDim.x * V) {
+    const int d0 = blockIdx.y * cols, d1 = min(a.H, d0 + cols);
+    for (int d = d0 + threadIdx.x * V; d < d1; d += blockDim.x * V) {
         float f[KT][V], x[V], o[V];
         if (a.R > 0) {      // a route without a row reads row 0, which is left out below
 #pragma unroll
@@ -483,8 +485,15 @@ template <bool RB, bool XB, int V>
 void sort_grad_k(hipStream_t st, const SortGradArgs& a) {
     // less than a work-group a CU: larger ones (8 slots of 7168: 32 tokens 11.5 ->
     // 8.0 us, 255 15.1 -> 11.8; 512 21.1 -> 22.4)
-    const int threads = a.T < kCus && a.H > kThreads * V ? 1024 : kThreads;
-#define GRIM_GRAD(KT) hipLaunchKernelGGL((sort_grad_kernel<RB, XB, KT, V>), dim3(a.T), dim3(threads), 0, st, a)
+    const int threads = a.w && a.T < kCus && a.H > kThreads * V ? 1024 : kThreads;
+    // without sums over the columns these are shared out until there are two
+    // work-groups a CU (32 tokens x 8 of 7168 in one work-group each 6.1 us, in
+    // four 4.8; 128: 7.3 and 6.4)
+    const int most = (a.H + kThreads * V - 1) / (kThreads * V);
+    const int parts = a.w || a.T >= 2 * kCus ? 1 : most < 2 * kCus / a.T ? most : 2 * kCus / a.T;
+    const int cols = ((a.H + parts - 1) / parts + V - 1) / V * V;
+    const dim3 grid(a.T, (a.H + cols - 1) / cols);
+#define GRIM_GRAD(KT) hipLaunchKernelGGL((sort_grad_kernel<RB, XB, KT, V>), grid, dim3(threads), 0, st, a, cols)
     if (a.K <= 1) GRIM_GRAD(1);
     else if (a.K <= 2) GRIM_GRAD(2);
     else if (a.K <= 4) GRIM_GRAD(4);

@@ -6,7 +6,7 @@ import torch
 
 from grimoire_amd import ops
 from test_gpu_proj4 import check, make_weight, reference, rows, run
-from test_gpu_sort_rows import check_combine, check_sort, data, routes, sort
+from test_gpu_sort_rows import check_combine, check_sort, check_sort_grad, data, routes, sort
 
 pytestmark = pytest.mark.gpu
 
@@ -32,6 +32,23 @@ def test_sort_sizes(gpu, T, E, K, H):
 def test_combine_slots(gpu, T, K):
     check_combine(gpu, T, K, 260, K, shared="bf16", gate=True)
     check_combine(gpu, T, K, 1032, K, dy_bf16=True, rows_bf16=False)
+
+
+@pytest.mark.parametrize("T", [1, 3, 100, 255, 256, 257, 511, 512])
+@pytest.mark.parametrize("H", [4, 1028, 7168])
+def test_sort_grad_columns(gpu, T, H):
+    """Columns shared out (without weights), larger work-groups (with)."""
+    K = 5
+    inv = torch.randperm(T * K, generator=torch.Generator().manual_seed(T)).int().view(T, K)
+    x, w = data(T, H, K, H)
+    drows = torch.randn((T * K, H), generator=torch.Generator().manual_seed(H)).bfloat16()
+    obj = ops.TokenSort(8, K, T, device=gpu)
+    for weighted in (False, True):
+        dx, dw = torch.full((T, H), float("nan"), device=gpu), torch.full((T, K), float("nan"), device=gpu)
+        kw = dict(x=x.to(gpu), weight=w.to(gpu), dweight=dw) if weighted else {}
+        obj.grad(drows.to(gpu), inv.to(gpu), dx, **kw)
+        torch.cuda.synchronize()
+        check_sort_grad(dx.cpu(), dw.cpu(), drows, inv, x, w if weighted else None)
 
 
 @pytest.mark.parametrize("T,E,K", [(6, 16, 4), (1100, 16, 8), (9000, 16, 8)])
