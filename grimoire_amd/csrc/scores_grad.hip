@@ -6,7 +6,10 @@
 //   softmax:  dl_e = s_e ([e picked] du_e - sum_k u_k du_k);  renormalised the
 //             sum is 0 and dl_k = p_k (g_k - sum_j p_j g_j), p the softmax of
 //             the picks alone: the other logits are not read
-//   sigmoid:  dl_e = s_e (1 - s_e) [e picked] du_e
+//   sigmoid:  dl_e = s_e (1 - s_e) [e picked] du_e;  renormalised
+//             dl_k = p_k (1 - s_k) (g_k - sum_j p_j g_j), p by the differences of
+//             the scores' exponents: Z, which may be any small number, is not
+//             divided by (scores of logits below -84 have a 1 / Z near fp32's largest)
 // The choice, and with it a selection bias and groups, has no gradient.  An
 // expert picked twice gets the sum, picks in order.  An expert that is out
 // (logit NaN or -inf) has score and gradient 0; +inf counts as the largest
@@ -42,6 +45,19 @@ __device__ __forceinline__ float wave_max(float v) {
     for (int o = 1; o < kWave; o <<= 1) v = fmaxf(v, __shfl_xor(v, o, kWave));
     return v;
 }
+
+// The largest of a row of 16 lanes, on each of them.
+__device__ __forceinline__ float row_max(float v) {
+    v = fmaxf(v, dpp_f<kDppXor1>(v));
+    v = fmaxf(v, dpp_f<kDppXor2>(v));
+    v = fmaxf(v, dpp_f<kDppHalfMirror>(v));
+    return fmaxf(v, dpp_f<kDppMirror>(v));
+}
+static_assert(kScoresMaxK == 16, "a token's picks are one row");
+
+// Where every pick's logit is at or below this, their sigmoids are 0 in the 64 bits
+// of the forward pass (e^709.783 > 2^1024), whose weights are 0 then.
+constexpr float kNoScores = -709.7827f;
 
 // exp(x), x <= 0: 2^(hi + lo) of x log2(e) in two parts, 1 - 2 ulp
 __device__ __forceinline__ float exp_neg(float x) {
@@ -105,16 +121,18 @@ __global__ __launch_bounds__(kWaves * kWave) void scores_grad_kernel(ScoresGradA
         const float p = z > 0.0f ? e / z : 0.0f;
         d = p * (g - group_sum<kWave>(p * g));
     } else {
-        // s = 1 / (1 + e^-l), s (1 - s) = e^-|l| / (1 + e^-|l|)^2
+        // s = e^min(l, 0) / (1 + e^-|l|), 1 - s = e^min(-l, 0) / (1 + e^-|l|)
         const float e = exp_neg(-__builtin_fabsf(pl)), q = 1.0f / (1.0f + e);
-        u = id >= 0 ? (pl >= 0.0f ? q : e * q) : 0.0f;
-        float du = g;
         if (a.normalize) {
-            const float z = group_sum<kWave>(u);
-            const float r = z > 0.0f ? 1.0f / z : 0.0f;
-            du = (g - group_sum<kWave>(u * r * g)) * r;
+            // the picks lie in the first 16 lanes: nothing comes from the others
+            const float low = fminf(pl, 0.0f), top = row_max(low);
+            u = id >= 0 && top > kNoScores ? exp_neg(low - top) * q : 0.0f;
+            const float z = group_sum<kScoresMaxK>(u);
+            const float p = z > 0.0f ? u / z : 0.0f;
+            d = p * (pl >= 0.0f ? e * q : q) * (g - group_sum<kScoresMaxK>(p * g));
+        } else {
+            d = e * q * q * g;
         }
-        d = e * q * q * du;
     }
     // an expert's picks summed by the first of them
     float tot = 0.0f;

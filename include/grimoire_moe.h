@@ -212,7 +212,9 @@ int grimoire_moe_router_scores(void* stream, const grim_score_params* p, const v
  *   else du_k = g_k.
  *   softmax: dlogits_e = s_e ([e picked] du_e - sum_k u_k du_k) (with
  *   normalize the sum is 0: exact zeros where nothing was picked);
- *   sigmoid: s_e (1 - s_e) [e picked] du_e.
+ *   sigmoid: s_e (1 - s_e) [e picked] du_e.  With normalize it is formed as
+ *   p_e (1 - s_e) (g_e - sum_j p_j g_j), however small Z is; only where the
+ *   weights themselves are 0 (every pick's logit below -709.78) it is 0.
  * The choice has no gradient: bias and groups in p are not read.  Picks
  * outside [0, n_experts) (slots no expert was left for) are left out, an
  * expert picked twice gets the sum.  An expert whose logit is NaN or -inf has
