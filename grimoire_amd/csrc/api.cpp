@@ -654,7 +654,8 @@ static int route_shape(int tokens, int top_k, int hidden) {
 }
 
 size_t grimoire_moe_sort_workspace_bytes(int tokens, int top_k, int num_experts) {
-    return sort_rows_workspace_bytes(tokens, top_k, num_experts);
+    const bool there = tokens >= 0 && top_k > 0 && top_k <= 16 && num_experts > 0 && num_experts <= kSortMaxE;
+    return there ? sort_rows_workspace_bytes(tokens, top_k, num_experts) : 0;
 }
 
 int grimoire_moe_sort_rows(void* stream, const int32_t* ids, const void* x, int x_bf16, int64_t x_stride,

@@ -559,6 +559,9 @@ class TokenSort:
     def __init__(self, num_experts: int, top_k: int, max_tokens: int, device="cuda"):
         self.num_experts, self.top_k, self.max_tokens = num_experts, top_k, max_tokens
         nbytes = int(lib().grimoire_moe_sort_workspace_bytes(max_tokens, top_k, num_experts))
+        if not nbytes:
+            raise _abi.GrimoireError(f"num_experts={num_experts} (1..16384), top_k={top_k} (1..16), "
+                                     f"max_tokens={max_tokens} (>= 0)")
         self._workspace = torch.empty(nbytes, dtype=torch.uint8, device=device)
         _dev(self._workspace)
         self.dev = self._workspace.get_device()

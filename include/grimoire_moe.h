@@ -380,7 +380,8 @@ int grimoire_moe_combine(void* stream, const uint16_t* src, const int32_t* inver
  * multiple of 8, bf16 is accessed 16 bytes at a time).  No output overlaps
  * another argument.  sort_rows takes a workspace (4-byte aligned, no initial
  * contents; calls that share one must not overlap) of
- * grimoire_moe_sort_workspace_bytes for up to `tokens` tokens. */
+ * grimoire_moe_sort_workspace_bytes for up to `tokens` tokens (0 for a top_k or
+ * num_experts that sort_rows refuses: 1 to 16, 1 to 16384). */
 size_t grimoire_moe_sort_workspace_bytes(int tokens, int top_k, int num_experts);
 int grimoire_moe_sort_rows(void* stream, const int32_t* ids, const void* x, int x_bf16, int64_t x_stride,
                            const float* weight, void* rows, int rows_bf16, int32_t* counts,
