@@ -324,7 +324,8 @@ __global__ __launch_bounds__(kWaves * 64, 4) void proj4_kernel(Proj4Dev p) {
 #pragma unroll
         for (int c = 0; c < CT; ++c) acc[c] = f32x4{0.f, 0.f, 0.f, 0.f};
         for (int s0 = 0; s0 < KB; s0 += p.slab) {
-            if (p.slab < KB && (s0 || set != set0)) {
+            // (a work-group goes on to other tiles only where all of its x stays)
+            if (s0) {
                 __syncthreads();                       // x of the slab before is not read any more
                 stage(kb0 + s0, min(p.slab, KB - s0), wave);
             }
@@ -480,7 +481,7 @@ hipError_t proj4_go(hipStream_t st, Proj4Dev& p) {
     if (lds > kLdsMost) return hipErrorInvalidValue;
     const bool again = p.slab >= p.kw_blocks && p.col_tiles == 1 && p.kw == 1;   // x stays for the next weights
     p.stride = again ? std::min(p.sets, 2 * kCus) : p.sets;
-    if (p.kw > 65535 || p.col_tiles > 65535) return hipErrorInvalidValue;
+    if (p.col_tiles > 65535) return hipErrorInvalidValue;
     const dim3 grid(unsigned(up(p.stride, 8)) * 8, p.kw, p.col_tiles);
     hipLaunchKernelGGL((proj4_kernel<GS, XB, CT>), grid, dim3(kWaves * 64), lds, st, p);
     return p.kw > 1 ? proj4_sum_launch(st, p) : hipGetLastError();
