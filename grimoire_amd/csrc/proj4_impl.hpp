@@ -101,6 +101,18 @@ __device__ __forceinline__ void put_chunk(uint8_t* to, u32x4 lo, u32x4 hi, bool 
             for (int k = 0; k < 4; ++k)
                 v[k] = GS == 0 ? tops(f_bits(f[2 * k + 1]), f_bits(f[2 * k])) : tops(f_bits(f[k + 4]), f_bits(f[k]));
             *reinterpret_cast<u32x4*>(to + l * 16) = v;
+            if constexpr (GS == 0) {
+                // MXFP4 products keep an infinity: its other pieces are 0.  One
+                // test of a chunk (of each element: 32 rows of 2880 x 5760 17.7 ->
+                // 18.7 us)
+                float most = 0.0f;
+#pragma unroll
+                for (int k = 0; k < 8; ++k) most = fmaxf(most, __builtin_fabsf(f[k]));
+                if (l == 0 && __builtin_expect(most == __builtin_inff(), 0)) {
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) f[k] = __builtin_fabsf(f[k]) == __builtin_inff() ? 0.0f : f[k];
+                }
+            }
             if (l < 2)
 #pragma unroll
                 for (int k = 0; k < 8; ++k) f[k] = rest(f[k]);

@@ -536,7 +536,8 @@ int grimoire_lora_swiglu(void* stream, const grim_lora* L, const int32_t* row_sl
  * base (same type and stride) and overlaps nothing else; rows at one distance
  * may lie beside each other in one buffer.  Codes and fp32 or bf16 activations
  * are multiplied exactly, sums are fp32.  A row of x with an infinity or a NaN
- * gives NaN or infinities in its own row alone; finite x should stay below
+ * changes its own row alone: MXFP4 as the formula has it, INT4 to NaN (the zero
+ * points come off with the sum of x); finite x should stay below
  * 5e33 (codes are multiplied as 16 + q).  Up to 2^18 rows; the weights are
  * read again for every 32 (bf16) or 8 (fp32) of them.
  * The workspace holds grimoire_proj4_workspace_bytes for up to `rows` rows
