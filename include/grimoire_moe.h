@@ -535,7 +535,13 @@ int grimoire_lora_swiglu(void* stream, const grim_lora* L, const int32_t* row_sl
  * elements apart (x a multiple of 8, 16-byte aligned; at most 2^28).  y may be
  * base (same type and stride) and overlaps nothing else; rows at one distance
  * may lie beside each other in one buffer.  Codes and fp32 or bf16 activations
- * are multiplied exactly, sums are fp32.  A row of x with an infinity or a NaN
+ * are multiplied exactly (bits of x below 2^-133 are not there), sums are fp32.
+ * INT4 takes the sums of (16 + q) x and of x apart: its rounding is relative to
+ * |s| (32 + q + z) |x|, not to |s (q - z) x|, and a group whose codes all equal
+ * their zero point leaves some in place of 0.  An MXFP4 weight is a bf16 number:
+ * above scale byte 252 the larger codes are infinities.  How K is shared out
+ * depends on the number of rows too, so a row's last bits may differ from batch
+ * to batch.  A row of x with an infinity or a NaN
  * changes its own row alone: MXFP4 as the formula has it, INT4 to NaN (the zero
  * points come off with the sum of x); finite x should stay below
  * 5e33 (codes are multiplied as 16 + q).  Up to 2^18 rows; the weights are

@@ -70,3 +70,43 @@ def test_swiglu_of_an_infinity(gpu, b16):
     ok = [0, 1, 3]
     want, tol = reference(w, x[ok], glu=True)
     check(y[ok], want, tol)
+
+
+@pytest.mark.parametrize("group", [32, 128])
+@pytest.mark.parametrize("b16", [False, True])
+def test_codes_at_their_zero_point(gpu, group, b16):
+    """The formula has 0: what is left is rounding of sums of (16 + q) x and x."""
+    w = make_weight("int4", "asym", 32, 1024, group, 7)
+    w.zeros.clamp_(max=15)
+    code = w.zeros.repeat_interleave(group // 2, dim=1)
+    w.payload.copy_(code | code << 4)
+    x = rows(6, 1024, 7, b16) + 2.0
+    v, tol = reference(w, x)
+    assert not v.any()
+    check(run(gpu, w, x), v, tol)
+
+
+@pytest.mark.parametrize("b16", [False, True])
+def test_largest_scales_of_mxfp4(gpu, b16):
+    """Scale byte 252 with every code, 254 with codes up to 1."""
+    w = make_weight("mxfp4", "none", 48, 128, 32, 9)
+    w.scales.fill_(252)
+    x = rows(5, 128, 9, b16) * 2.0 ** -30
+    check(run(gpu, w, x), *reference(w, x))
+    w.scales.fill_(254)
+    codes = torch.tensor([0, 1, 2, 8, 9, 10], dtype=torch.uint8)
+    w.payload.copy_(codes[(w.payload % 6).long()] | codes[(w.payload // 6 % 6).long()] << 4)
+    assert dequant(w).abs().max() <= 2.0 ** 127
+    check(run(gpu, w, x), *reference(w, x))
+
+
+@pytest.mark.parametrize("b16,most", [(True, 16), (False, 4)])
+def test_rows_alone_and_in_a_batch(gpu, b16, most):
+    """The same bits where x of a whole row stays in the LDS for either, as K is
+    shared out alike then (wider rows: header)."""
+    for fmt in ("int4", "mxfp4"):
+        w = make_weight(fmt, "asym", 80, 1536, 128, 5)
+        x = rows(most, 1536, 5, b16)
+        y = run(gpu, w, x)
+        for t in (0, 1, most - 1):
+            assert torch.equal(run(gpu, w, x[t:t + 1]), y[t:t + 1])
