@@ -28,26 +28,16 @@
 // bf16 pieces of 8 significant bits, cut off, not rounded, so each rest is
 // exact; with bf16 weights every product is exact in the fp32 accumulator.
 #include "lora.hpp"
+#include "bf16_mfma.hpp"
 
 namespace grim {
 
 namespace {
 
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-
 constexpr int kRows = kLoraRows;
 constexpr int kStep = kLoraStep;     // 16 k a lane
 constexpr int kShrinkWaves = kLoraShrinkWaves;
 constexpr int kExpandWaves = 4;
-
-__device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
-    bf16x8 av, bv;
-    __builtin_memcpy(&av, &a, 16);
-    __builtin_memcpy(&bv, &b, 16);
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(av, bv, c, 0, 0, 0);
-}
 
 // v minus its top 16 bits: the rest of a cut to bf16 (0 for infinities,
 // whose first piece holds them; a NaN stays one)

@@ -15,6 +15,7 @@
 // registers, and 64 rows of 4096 x 8192 took 30.8 us where twos take 21.7.
 #pragma once
 
+#include "bf16_mfma.hpp"
 #include "proj4_out.hpp"
 
 #include <algorithm>
@@ -23,24 +24,14 @@ namespace grim {
 
 namespace {
 
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-
 constexpr int kBlk = 128;                 // k of a block: 16 bytes a lane, 4 lanes a weight row
 constexpr int kChunks = kBlk / 8;         // its chunks of 8 k
 constexpr int kSeg = 4;                   // blocks in flight
 constexpr int kWaves = 8;                 // of a work-group
 
-__device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
-    bf16x8 av, bv;
-    __builtin_memcpy(&av, &a, 16);
-    __builtin_memcpy(&bv, &b, 16);
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(av, bv, c, 0, 0, 0);
-}
-
-// v minus its top 16 bits: the rest of a cut to bf16 (exact; NaN for an infinity)
-__device__ __forceinline__ float rest(float v) { return v - bits_f(f_bits(v) & 0xFFFF0000u); }
+// v, finite, minus its top 16 bits: the rest of a cut to bf16, exact (an
+// infinity's is NaN, which INT4 products come to anyway)
+__device__ __forceinline__ float rest_of_finite(float v) { return v - bits_f(f_bits(v) & 0xFFFF0000u); }
 // the top / bottom halves of two words: {hi, lo}
 __device__ __forceinline__ uint32_t tops(uint32_t hi, uint32_t lo) { return __builtin_amdgcn_perm(hi, lo, 0x07060302u); }
 __device__ __forceinline__ uint32_t bottoms(uint32_t hi, uint32_t lo) { return __builtin_amdgcn_perm(hi, lo, 0x05040100u); }
@@ -115,7 +106,7 @@ __device__ __forceinline__ void put_chunk(uint8_t* to, u32x4 lo, u32x4 hi, bool 
             }
             if (l < 2)
 #pragma unroll
-                for (int k = 0; k < 8; ++k) f[k] = rest(f[k]);
+                for (int k = 0; k < 8; ++k) f[k] = rest_of_finite(f[k]);
         }
     }
 }
