@@ -3,7 +3,7 @@
 // (MXFP4: sum_g 2^(e[n,g] - 127) sum_k e2m1[n,k] x_t[k]), optionally with the
 // SwiGLU of a gate|up projection.
 //
-// The weights are read once, 4.13 (groups of 128) to 4.75 bits an element (of 32,
+// The weights are read once, 4.06 (groups of 256) to 4.75 bits an element (of 32,
 // with zeros), and bound a few rows: 7168 x 32768 is 123 MB, 24 us at a copy's
 // 5.1 TB/s.  Products go to the matrix cores with x as rows and
 // the decoded weights as columns: x's 16 rows (bf16) cost what one does.  fp32 x
@@ -14,13 +14,14 @@
 // with ones gives; the scale is applied to that sum in fp32.  MXFP4: the
 // conversion instruction gives w s in bf16, exact.  Sums are fp32.
 //
-// What bounds it now (kernel alone, weights in no cache): one row of 7168 x
-// 32768 INT4 31 us, 4.0 TB/s, 78 % of a copy's rate; its loads alone take 30, the
-// decoding alone (51 to 84 vector operations for 1 KiB of codes and 64 lanes) 23,
-// x and the launch 4 of either.  Small ones are chains: 768 x 2048 5.2
-// us, 2880 x 5760 with SwiGLU for 8 rows 8.2 (fetch x, LDS, the first weights, the
-// sum over the waves).  32 rows of 7168 x 4096 with SwiGLU 16.1 us: 58 KB of x a
-// part of K in each work-group, and the second launch that sums.
+// What bounds it now: one row of 7168 x 32768 INT4, weights in no cache, 29 us,
+// 4.2 TB/s, 83 % of a copy's rate; its loads alone take as long, the decoding alone
+// (51 to 84 vector operations for 1 KiB of codes and 64 lanes) three quarters,
+// x and the launch 4 of either.  Small ones are chains: 768 x 2048 5 us, 2880 x 5760
+// with SwiGLU for 8 rows 7 (fetch x, LDS, the first weights, the sum over the
+// waves).  32 rows of 7168 x 4096 with SwiGLU 14 us: 58 KB of x a part of K in each
+// work-group, and the second launch that sums (of bf16 x; of fp32, 8 rows a
+// work-group, 26).
 #include "proj4_out.hpp"
 
 namespace grim {

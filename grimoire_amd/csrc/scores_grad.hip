@@ -15,8 +15,9 @@
 // (logit NaN or -inf) has score and gradient 0; +inf counts as the largest
 // finite logit, as in the scores.  All is fp32; an exponential is off by 2 ulp.
 //
-// Bound by the launch at a step's sizes (4096 x 128 fp32, 4 MB: 2 us at a copy's
-// rate, 7.8 a call of which the host takes 5.6).  A wave holds a token's logits in
+// Bound by latency (4096 x 128 fp32, softmax kept, 4.5 MB, 0.9 us at a large copy's
+// 5.1 TB/s: 4.1 in a graph, 6.2 a call, the host's; 64 x 256 sigmoid 3.0 in a graph,
+// 4096 x 512 softmax kept, 17 MB, 6 to 8; one token 2.4).  A wave holds a token's logits in
 // registers, 1 to 8 a lane as E needs, so that each is read once and every sum
 // is one of lanes; the picks lie one a lane.  Renormalised softmax reads the
 // picks' logits alone.  The picks' values go to their experts' places through a
